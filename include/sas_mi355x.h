@@ -20,6 +20,9 @@
  *   sas_kv_fp8_append      <- no counterpart in the reference (its caches are bf16/fp16 only,
  *                             api.py:51-56): writer of the fp8 cache-row format that
  *                             SAS_KV_FP8_DS_MLA selects for sas_attention_launch.
+ *   sas_norm_rope, sas_kv_append_rope, sas_topk_select
+ *                          <- no counterpart either: the queries, cache rows and row ids that
+ *                             the reference takes as inputs.
  */
 #ifndef SAS_MI355X_H_
 #define SAS_MI355X_H_
@@ -275,6 +278,87 @@ int sas_attention_launch_noalloc(const SasAttnArgs* args, void* stream);
  * SAS_E_INVALID for a null pointer or n < 0. */
 int sas_kv_fp8_append(const void* src, const int32_t* slot_mapping, void* cache, int n,
                       int64_t cache_rows, void* stream);
+
+/* ---- row operators: norm, rotation, cache append (no reference counterpart) ----------
+ * The reference takes rotated queries and written caches as inputs (api.py:129-153); these
+ * make them. A row x of `dim` elements becomes, in fp32 and rounded once at the end,
+ *   y[d] = x[d] * w[d] / sqrt(mean(x[0..norm_dim)^2) + eps)  for d < norm_dim, else x[d],
+ * then the pairs of dims [rope_offset, rope_offset + rope_dim) turn by the angles of the row's
+ * position: (a, b) -> (a cos - b sin, b cos + a sin), pair i being dims (2i, 2i + 1) of the
+ * range (interleaved != 0) or (i, i + rope_dim / 2). A position outside the table gives NaN
+ * in the rotated dims.
+ *
+ * Row formats: SAS_ROW_NATIVE, dim elements of `dtype`; SAS_ROW_FP8_DS_MLA, the 656-byte rows of
+ * SAS_KV_FP8_DS_MLA; SAS_ROW_FP8_INDEX, for index keys: a page of block_size rows is their
+ * block_size * dim e4m3 codes, then their block_size fp32 scales (amax / 448, 1 for a zero row).
+ * A row with a non-finite value to quantize gets a NaN scale. */
+#define SAS_ROW_NATIVE 0
+#define SAS_ROW_FP8_DS_MLA 1
+#define SAS_ROW_FP8_INDEX 2
+#define SAS_ROW_MAX_DIM 1024
+
+typedef struct SasRowArgs {
+  const void* x;            /* rows, 16-byte aligned; element strides below, multiples of 8       */
+  void* out;                /* sas_norm_rope: rows (x itself is allowed); append: the cache       */
+  const int32_t* positions; /* [tokens], or NULL if rope_dim == 0                                 */
+  const float* cos_sin;     /* [max_position, rope_dim]: rope_dim / 2 cosines, then the sines     */
+  const void* norm_weight;  /* [norm_dim], or NULL if norm_dim == 0                               */
+  const int32_t* slots;     /* append: [tokens] flat cache row; outside [0, cache_rows): skipped  */
+  int64_t x_token_stride, x_head_stride, out_token_stride, out_head_stride;
+  int64_t cache_rows;
+  int32_t tokens, heads, dim, norm_dim, rope_dim, rope_offset;
+  int32_t interleaved, max_position, dtype, norm_weight_fp32;  /* weight: fp32, else `dtype`      */
+  int32_t row_format, block_size;                              /* append (block_size: fp8 index)  */
+  float eps;
+  int32_t reserved;
+} SasRowArgs;
+
+/* Norm and rotation of the heads of `tokens` tokens. dim, norm_dim and rope_offset are multiples
+ * of 8, rope_dim of 8 (interleaved) or 16. Asynchronous on `stream`. */
+int sas_norm_rope(const SasRowArgs* args, void* stream);
+
+/* The same of `tokens` rows (heads = 1) on their way into a paged cache. Two rows with one slot
+ * leave unspecified contents there. SAS_ROW_FP8_DS_MLA: dim 576, bf16; SAS_ROW_FP8_INDEX: dim 64
+ * or 128, block_size * (dim + 4) a multiple of 16, cache_rows whole pages. */
+int sas_kv_append_rope(const SasRowArgs* args, void* stream);
+int sas_row_args_struct_size(void);
+
+/* ---- choosing the rows to attend (no reference counterpart: cmp_sparse_indices is an input of
+ * the reference, api.py:137) ------------------------------------------------------------------
+ * Query row t at causal position p of its sequence (the last row is at seqused_kv - 1) scores
+ * index keys j < min((p + 1) / cmp_ratio, max_keys) of the paged index cache:
+ *   s(t, j) = scale_j * sum_h weights[t, h] * max(0, q[t, h] . k[j])
+ * and out[t] holds the ids of the topk largest in ascending order, -1 behind them: an input of
+ * SasAttnArgs.cmp_indices. The choice is that of scores in 64 bits (equal ones: the lowest ids),
+ * whatever the batch and the split of the work; NaN scores rank lowest. Keys on a page outside
+ * [0, block_num) are never chosen, rows of no sequence get -1. Launches kernels only; the
+ * workspace (sas_topk_select_workspace bytes, 16-byte aligned, contents ignored) belongs to the
+ * call until it has run. */
+#define SAS_SELECT_MAX_HEADS 128
+#define SAS_SELECT_MAX_KEYS (1 << 24)
+
+typedef struct SasSelectArgs {
+  const void* q;              /* [tokens, heads, dim] dtype                                       */
+  const float* weights;       /* [tokens, heads]                                                  */
+  const void* keys;           /* [block_num, block_size, dim] dtype, or fp8 index pages           */
+  const int32_t* block_table; /* [batch, table_len]                                               */
+  const int32_t* cu_seqlens_q;/* [batch + 1] non-decreasing, or NULL with rows_per_seq            */
+  const int32_t* seqused_kv;  /* [batch] raw length of each sequence                              */
+  int32_t* out;               /* [tokens, topk]                                                   */
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t batch, tokens;
+  int32_t rows_per_seq;       /* 0: rows by cu_seqlens_q. Else sequence b owns rows [b, b + 1) *
+                               * rows_per_seq, of which the first cu_seqlens_q[b + 1] -
+                               * cu_seqlens_q[b] are in use (all of them if it is NULL)           */
+  int32_t heads, dim, topk, cmp_ratio;
+  int32_t block_num, block_size, table_len, max_keys, dtype, key_format;
+} SasSelectArgs;
+
+/* Workspace of a call with these sizes (pointers ignored), or -1 (see sas_last_error). */
+int64_t sas_topk_select_workspace(const SasSelectArgs* args);
+int sas_topk_select(const SasSelectArgs* args, void* stream);
+int sas_select_args_struct_size(void);
 
 /* Library version (major * 100 + minor). */
 int sas_version(void);

@@ -33,6 +33,12 @@ DTYPE_FP16 = 1
 KV_NATIVE = 0
 KV_FP8_DS_MLA = 1
 FP8_ROW_BYTES = 656
+ROW_NATIVE = 0                # SasRowArgs.row_format, SasSelectArgs.key_format
+ROW_FP8_DS_MLA = 1
+ROW_FP8_INDEX = 2
+ROW_MAX_DIM = 1024
+SELECT_MAX_HEADS = 128
+SELECT_MAX_KEYS = 1 << 24
 SAS_PHASE_PIPELINED = 4        # SasAttnArgs.phases bit: native rows through the pipelined kernel
 SAS_PHASE_FP8_QK = 8           # SasAttnArgs.phases bit: fp8 rows, Q·Kᵀ on fp8 MFMA (e4m3 queries)
 SAS_PHASE_ROW_ITEMS = 16       # SasAttnArgs.phases bit: no row pairs (one query row per item)
@@ -91,9 +97,38 @@ class SasAttnArgs(ctypes.Structure):
     ]
 
 
+class SasRowArgs(ctypes.Structure):
+    """Field-for-field mirror of ``SasRowArgs`` in ``include/sas_mi355x.h``."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "out", "positions", "cos_sin", "norm_weight",
+                                                "slots")] +
+                [(n, ctypes.c_int64) for n in ("x_token_stride", "x_head_stride",
+                                               "out_token_stride", "out_head_stride",
+                                               "cache_rows")] +
+                [(n, ctypes.c_int32) for n in ("tokens", "heads", "dim", "norm_dim", "rope_dim",
+                                               "rope_offset", "interleaved", "max_position",
+                                               "dtype", "norm_weight_fp32", "row_format",
+                                               "block_size")] +
+                [("eps", ctypes.c_float), ("reserved", ctypes.c_int32)])
+
+
+class SasSelectArgs(ctypes.Structure):
+    """Field-for-field mirror of ``SasSelectArgs`` in ``include/sas_mi355x.h``."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "weights", "keys", "block_table",
+                                                "cu_seqlens_q", "seqused_kv", "out",
+                                                "workspace")] +
+                [("workspace_bytes", ctypes.c_int64)] +
+                [(n, ctypes.c_int32) for n in ("batch", "tokens", "rows_per_seq", "heads", "dim",
+                                               "topk", "cmp_ratio", "block_num", "block_size",
+                                               "table_len", "max_keys", "dtype", "key_format")])
+
+
 EXPORTS = ("sas_metadata_build", "sas_metadata_build_device", "sas_metadata_build_device_cu",
            "sas_workspace_bytes", "sas_attention_launch", "sas_attention_launch_lens",
            "sas_attention_launch_noalloc", "sas_merge_sync_take", "sas_kv_fp8_append",
+           "sas_norm_rope", "sas_kv_append_rope", "sas_row_args_struct_size",
+           "sas_topk_select", "sas_topk_select_workspace", "sas_select_args_struct_size",
            "sas_version", "sas_args_struct_size", "sas_last_error")
 NOALLOC_SCRATCH_BYTES = 72 << 20  # SAS_NOALLOC_SCRATCH_BYTES
 
@@ -139,11 +174,23 @@ def load() -> ctypes.CDLL:
         lib.sas_kv_fp8_append.restype = ctypes.c_int
         lib.sas_kv_fp8_append.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                           ctypes.c_int, ctypes.c_int64, ctypes.c_void_p]
+        for entry in (lib.sas_norm_rope, lib.sas_kv_append_rope):
+            entry.restype = ctypes.c_int
+            entry.argtypes = [ctypes.POINTER(SasRowArgs), ctypes.c_void_p]
+        lib.sas_topk_select.restype = ctypes.c_int
+        lib.sas_topk_select.argtypes = [ctypes.POINTER(SasSelectArgs), ctypes.c_void_p]
+        lib.sas_topk_select_workspace.restype = ctypes.c_int64
+        lib.sas_topk_select_workspace.argtypes = [ctypes.POINTER(SasSelectArgs)]
+        lib.sas_row_args_struct_size.restype = ctypes.c_int
+        lib.sas_select_args_struct_size.restype = ctypes.c_int
         lib.sas_version.restype = ctypes.c_int
         lib.sas_args_struct_size.restype = ctypes.c_int
         lib.sas_last_error.restype = ctypes.c_char_p
         if lib.sas_args_struct_size() != ctypes.sizeof(SasAttnArgs):
             raise RuntimeError("SasAttnArgs layout mismatch between the library and its binding")
+        if (lib.sas_row_args_struct_size() != ctypes.sizeof(SasRowArgs)
+                or lib.sas_select_args_struct_size() != ctypes.sizeof(SasSelectArgs)):
+            raise RuntimeError("argument layout mismatch between the library and its binding")
         _lib = lib
     return _lib
 

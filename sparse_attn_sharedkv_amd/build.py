@@ -17,7 +17,8 @@ ROOT = os.path.dirname(PKG)
 LIB_DIR = os.path.join(PKG, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libsas_mi355x.so")
 SOURCES = [os.path.join(PKG, "csrc", n) for n in ("sas_attn.hip", "sas_kv_fp8.hip", "sas_metadata.cpp",
-                                                   "sas_metadata_dev.hip")]
+                                                   "sas_metadata_dev.hip", "sas_rows.hip",
+                                                   "sas_select.hip")]
 HIP_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
     # packed FP32 VALU forms are kept out of generated code on this target
