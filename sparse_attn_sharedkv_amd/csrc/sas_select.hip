@@ -41,6 +41,7 @@ void set_error(const std::string& msg);
 namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef double f64x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -100,7 +101,7 @@ __device__ inline u32x4 widen_e4m3(u32x2 c) {
 struct SelPlan {
   int t_begin, t_end;   // query rows of this pass
   int width;            // scores kept for a row (row stride of the workspace)
-  int chunk, chunks;    // keys of a workgroup, and such pieces in `width`
+  int chunks;           // workgroups that share a row's keys
   int slices;           // waves that share a chunk's keys (each leaves its own key norm)
   int wq;               // query rows of a workgroup
   FastDiv page_div, ratio_div;
@@ -155,9 +156,16 @@ __device__ inline RowPos locate(const SasSelectArgs& a, const SelPlan& p, int t)
   return r;
 }
 
-// thr of the last row before `end` that belongs to the same sequence as a row with `thr` at `t`.
 __device__ inline int thr_at(const SasSelectArgs& a, const SelPlan& p, int t) {
   return locate(a, p, t).thr;
+}
+
+// Keys of one of a row's pieces: equal shares of the keys it has, in whole steps of 64 keys a
+// slice, so no workgroup of a short sequence in a wide table goes without work before the
+// last pieces do.
+__device__ inline int piece_keys(const SelPlan& p, int thr) {
+  const int unit = 64 * p.slices;
+  return ((thr + p.chunks - 1) / p.chunks + unit - 1) / unit * unit;
 }
 
 // ---------------------------------------------------------------------------
@@ -269,9 +277,9 @@ __global__ __launch_bounds__(256) void score_stream_kernel(SasSelectArgs a, SelP
   const int t = p.t_begin + (int)(blockIdx.x / (unsigned)p.chunks) * p.wq + wave % p.wq;
   if (t >= p.t_end) return;
   const RowPos r = locate(a, p, t);
-  const int lo = piece * p.chunk;
+  const int keys = piece_keys(p, r.thr), lo = piece * keys;
   if (r.b < 0 || r.thr <= a.topk || lo >= r.thr) return;
-  const int hi = min(lo + p.chunk, r.thr), slice = wave / p.wq, step = 32 * p.slices;
+  const int hi = min(lo + keys, r.thr), slice = wave / p.wq, step = 32 * p.slices;
 
   QueryFrags<T, D, MT> qf;
   qf.load(a, t, lane);
@@ -368,7 +376,6 @@ __global__ __launch_bounds__(64 * TILE_WAVES) void score_tile_kernel(SasSelectAr
   // the last rows of a causal prefill have the most keys: they start first
   const int t0 = p.t_begin + (tiles - 1 - (int)(blockIdx.x / (unsigned)p.chunks)) * TILE_WAVES;
   const int t1 = min(t0 + TILE_WAVES, p.t_end), t = t0 + wave;
-  const int lo = piece * p.chunk;
   // the thread's part of a stage: bytes [32 part, +32) of native row `row`, or 16 codes
   constexpr int PARTS = 64 * TILE_WAVES / TILE_KEYS;   // 8 threads a row
   constexpr int LOADS = FP8 ? 1 : D * 2 / (16 * PARTS);  // 16-byte loads of a thread
@@ -380,7 +387,7 @@ __global__ __launch_bounds__(64 * TILE_WAVES) void score_tile_kernel(SasSelectAr
     const RowPos seg = locate(a, p, ts);
     const int te = max(min(seg.last, t1), ts + 1);
     const int thr_end = seg.b < 0 ? 0 : thr_at(a, p, te - 1);
-    const int hi = min(lo + p.chunk, thr_end);
+    const int keys = piece_keys(p, thr_end), lo = piece * keys, hi = min(lo + keys, thr_end);
     if (thr_end <= a.topk || lo >= thr_end) {
       ts = te;
       continue;
@@ -482,19 +489,34 @@ __global__ __launch_bounds__(64 * TILE_WAVES) void score_tile_kernel(SasSelectAr
 // ---------------------------------------------------------------------------
 // Selection
 // ---------------------------------------------------------------------------
+//
+// A workgroup for each query row. The row's scores (or, of a row too long for the registers, the
+// ones above a threshold that a sample puts a little below the topk-th) are in registers:
+//   1. the topk-th largest, by one histogram over their range and a ranking inside its bin;
+//   2. those above the bound are taken, those inside it scored in 64 bits and ranked;
+//   3. every id taken is a bit of a map in LDS, from which the ids come out in order.
+// Bound by the latency of these steps, not by bytes, so steps are few and long rows get many
+// waves, while the many short rows of a prefill get one wave each, which needs no barriers.
+// What does not fit (a bound that is not finite, more equal scores than the lists hold) goes
+// through select_from_memory: the same steps over the scores in memory, as often as it takes.
 
-constexpr int SEL_BINS = 2048;
-constexpr int SEL_LIST = 1024;  // rows scored again, or ranked, in LDS
+template <int THREADS>
+struct SelSize {
+  static constexpr int WAVES = THREADS / 64;
+  static constexpr int BINS = THREADS == 64 ? 512 : THREADS == 256 ? 1024 : 2048;
+  static constexpr int LIST = THREADS == 64 ? 128 : THREADS == 256 ? 256 : 1024;
+  static constexpr int PARTS = THREADS == 64 ? 1 : SAS_SELECT_MAX_HEADS / 16;
+};
 
-template <int THREADS, int ROWCAP>
+template <int THREADS>
 struct SelShared {
-  float row[ROWCAP > 0 ? ROWCAP : 1];
-  uint32_t bins[SEL_BINS];
-  float list_x[SEL_LIST];
-  int list_j[SEL_LIST];
-  uint64_t list_key[SEL_LIST];
-  int wave_a[THREADS / 64], wave_b[THREADS / 64];
-  float wave_lo[THREADS / 64], wave_hi[THREADS / 64];
+  typedef SelSize<THREADS> S;
+  uint32_t bins[S::BINS];
+  float list_x[S::LIST];
+  int list_j[S::LIST];
+  uint64_t list_key[S::LIST];
+  int wave_a[S::WAVES], wave_b[S::WAVES];
+  float wave_lo[S::WAVES], wave_hi[S::WAVES];
   int count, found, below, in_bin;
   float value;
 };
@@ -507,61 +529,92 @@ __device__ inline uint64_t order_of(double s) {
   return u >> 63 ? ~u : u | (1ull << 63);
 }
 
-// The score of key j in 64 bits, by one wave (the same in every lane): lanes are heads, and
-// where there are fewer than 64 several lanes share a head's dims.
+// Scores of 16 keys over 16 heads in 64 bits, by one wave: lane l is key l & 15 (`j`, any id of the
+// sequence) and holds a quarter of the dims of it and of head h0 + (l & 15), so that both operands
+// come in whole 16-byte loads; the dims are summed in the order the matrix instruction takes
+// them. Returns the heads' weighted sum for the lane's key without its scale, the same in its four
+// lanes. Element r of the product is head 4 r + l / 16.
 template <typename T, bool FP8>
-__device__ double score64(const SasSelectArgs& a, const SelPlan& p, int t, const int32_t* table, int j,
-                          int lane) {
-  const int d = a.dim;
-  int hp = 1;
-  while (hp < a.heads && hp < 64) hp <<= 1;
-  int parts = 64 / hp;
-  while (parts > d / 8) parts >>= 1;
-  const int dims = d / parts;  // a multiple of 8
-  const int part = lane / hp;
+__device__ inline double score64_part(const SasSelectArgs& a, const SelPlan& p, int t,
+                                      const int32_t* table, int j, int h0, int lane) {
+  const int d = a.dim, quarter = d / 4, c = lane & 15, kq = lane >> 4;
+  const int pg = p.page_div.div(j);
+  int64_t page = table[pg], at = j - pg * a.block_size;
+  if (page < 0 || page >= a.block_num) page = at = 0;  // (a key nobody asks for)
+  const int h = h0 + c;
+  const T* q = (const T*)a.q + ((int64_t)t * a.heads + min(h, a.heads - 1)) * d + kq * quarter;
+  u32x4 qv[4], kv[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (8 * i < quarter) qv[i] = *(const u32x4*)(q + 8 * i);
+  }
+  if (!FP8) {
+    const T* k = (const T*)a.keys + (page * a.block_size + at) * d + kq * quarter;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (8 * i < quarter) kv[i] = *(const u32x4*)(k + 8 * i);
+    }
+  } else {
+    const unsigned char* k = (const unsigned char*)a.keys + page * a.block_size * (d + 4) + at * d +
+                             kq * quarter;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (8 * i < quarter) kv[i] = widen_e4m3<T>(*(const u32x2*)(k + 8 * i));
+    }
+  }
+  double w[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int hh = h0 + 4 * r + kq;
+    w[r] = hh < a.heads ? (double)a.weights[(int64_t)t * a.heads + hh] : 0.0;
+  }
+  f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (8 * i >= quarter) break;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)Elem<T>::lo(qv[i][e]),
+                                                 (double)Elem<T>::lo(kv[i][e]), acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)Elem<T>::hi(qv[i][e]),
+                                                 (double)Elem<T>::hi(kv[i][e]), acc, 0, 0, 0);
+    }
+  }
+  double s = 0.0;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const double x = acc[r] < 0.0 ? 0.0 : acc[r];  // (keeps NaN)
+    if (h0 + 4 * r + kq < a.heads) s += x * w[r];
+  }
+  s += __shfl_xor(s, 16, 64);
+  return s + __shfl_xor(s, 32, 64);
+}
+
+template <bool FP8>
+__device__ inline double key_scale64(const SasSelectArgs& a, const SelPlan& p, const int32_t* table,
+                                     int j) {
+  if (!FP8) return 1.0;
   const int pg = p.page_div.div(j), at = j - pg * a.block_size;
   const int64_t page = table[pg];
-  const T* krow = nullptr;
-  const unsigned char* crow = nullptr;
-  double scale = 1.0;
-  if (!FP8) {
-    krow = (const T*)a.keys + (page * a.block_size + at) * d;
-  } else {
-    const unsigned char* base = (const unsigned char*)a.keys + page * a.block_size * (d + 4);
-    crow = base + (int64_t)at * d;
-    scale = (double)*(const float*)(base + (int64_t)a.block_size * d + 4 * at);
-  }
-  double total = 0.0;
-  for (int h0 = 0; h0 < a.heads; h0 += 64) {
-    const int h = h0 + (lane & (hp - 1));
-    const bool live = h < a.heads && part < parts;
-    double acc = 0.0;
-    if (live) {
-      const T* q = (const T*)a.q + ((int64_t)t * a.heads + h) * d + part * dims;
-      for (int e = 0; e < dims; e += 8) {
-        const u32x4 qv = *(const u32x4*)(q + e);
-        const u32x4 kv = FP8 ? widen_e4m3<T>(*(const u32x2*)(crow + part * dims + e))
-                             : *(const u32x4*)(krow + part * dims + e);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          acc = fma((double)Elem<T>::lo(qv[i]), (double)Elem<T>::lo(kv[i]), acc);
-          acc = fma((double)Elem<T>::hi(qv[i]), (double)Elem<T>::hi(kv[i]), acc);
-        }
-      }
-    }
-    for (int off = hp; off < hp * parts; off <<= 1) acc += __shfl_xor(acc, off, 64);
-    const double x = acc < 0.0 ? 0.0 : acc;  // (keeps NaN)
-    double s = live && part == 0 ? x * (double)a.weights[(int64_t)t * a.heads + h] : 0.0;
-    for (int off = 1; off < hp; off <<= 1) s += __shfl_xor(s, off, 64);
-    total += s;
-  }
-  return __shfl(total * scale, 0, 64);
+  if (page < 0 || page >= a.block_num) return 0.0;
+  return (double)*(const float*)((const unsigned char*)a.keys + page * a.block_size * (a.dim + 4) +
+                                 (int64_t)a.block_size * a.dim + 4 * at);
+}
+
+// Order of the scores of 16 keys (lane l: key `j`, l & 15), by one wave.
+template <typename T, bool FP8>
+__device__ inline uint64_t order64(const SasSelectArgs& a, const SelPlan& p, int t,
+                                   const int32_t* table, int j, int lane) {
+  double s = 0.0;
+  for (int h0 = 0; h0 < a.heads; h0 += 16) s += score64_part<T, FP8>(a, p, t, table, j, h0, lane);
+  return order_of(s * key_scale64<FP8>(a, p, table, j));
 }
 
 template <int THREADS>
 __device__ inline int block_sum(int v, int* scratch) {
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(v, off, 64);
+  if (THREADS == 64) return v;
   __syncthreads();
   if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -571,17 +624,102 @@ __device__ inline int block_sum(int v, int* scratch) {
   return s;
 }
 
-template <typename T, bool FP8, int THREADS, int ROWCAP>
-__global__ __launch_bounds__(THREADS) void select_kernel(SasSelectArgs a, SelPlan p) {
-  __shared__ SelShared<THREADS, ROWCAP> sh;
-  constexpr int WAVES = THREADS / 64;
+// The range of the workgroup's values, the same in every thread.
+template <int THREADS>
+__device__ inline void block_range(float& lo, float& hi, SelShared<THREADS>& sh) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    lo = fminf(lo, __shfl_xor(lo, off, 64));
+    hi = fmaxf(hi, __shfl_xor(hi, off, 64));
+  }
+  if (THREADS == 64) return;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    sh.wave_lo[threadIdx.x >> 6] = lo;
+    sh.wave_hi[threadIdx.x >> 6] = hi;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    lo = fminf(lo, sh.wave_lo[w]);
+    hi = fmaxf(hi, sh.wave_hi[w]);
+  }
+}
+
+// Sum of the threads' values before this one's; `all` is the sum of every thread's.
+template <int THREADS>
+__device__ inline int block_before(int v, int* scratch, int& all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int incl = v;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int u = __shfl_up(incl, off, 64);
+    if (lane >= off) incl += u;
+  }
+  if (THREADS == 64) {
+    all = __shfl(incl, 63, 64);
+    return incl - v;
+  }
+  __syncthreads();
+  if (lane == 63) scratch[wave] = incl;
+  __syncthreads();
+  int before = incl - v;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    before += w < wave ? scratch[w] : 0;
+    all += scratch[w];
+  }
+  return before;
+}
+
+// Finds the bin that holds the need-th value from the top: sh.found, the values above it
+// sh.below, and its own sh.in_bin. Ends with a barrier.
+template <int THREADS>
+__device__ inline void find_bin(int need, SelShared<THREADS>& sh) {
+  constexpr int BINS = SelSize<THREADS>::BINS, PER = BINS / THREADS;
+  int c[PER], sum = 0, all;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    c[i] = (int)sh.bins[BINS - 1 - ((int)threadIdx.x * PER + i)];
+    sum += c[i];
+  }
+  int before = block_before<THREADS>(sum, sh.wave_a, all);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (before < need && need <= before + c[i]) {
+      sh.found = BINS - 1 - ((int)threadIdx.x * PER + i);
+      sh.below = before;
+      sh.in_bin = c[i];
+    }
+    before += c[i];
+  }
+  __syncthreads();
+}
+
+// A monotone map of [lo, hi] onto the bins (values outside go below bin 0, or to the last).
+template <int THREADS>
+struct BinMap {
+  float base, inv;
+  __device__ static BinMap of(float lo, float hi) {
+    return {0.5f * lo, (float)(SelSize<THREADS>::BINS - 1) / (0.5f * hi - 0.5f * lo)};
+  }
+  __device__ bool usable() const { return inv < SEL_MAX; }
+  __device__ int bin(float x) const {
+    const float b = fminf((0.5f * x - base) * inv, (float)(SelSize<THREADS>::BINS - 1));
+    return b < 0.0f ? -1 : (int)b;
+  }
+};
+
+// The choice from scores in memory, for what the registers and lists do not hold.
+template <typename T, bool FP8, int THREADS>
+__device__ inline void select_from_memory(const SasSelectArgs& a, const SelPlan& p, int t, int n,
+                                                float err, float* x_of, const int32_t* table,
+                                                SelShared<THREADS>& sh) {
+  constexpr int WAVES = THREADS / 64, BINS = SelSize<THREADS>::BINS, LIST = SelSize<THREADS>::LIST;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int t = p.t_begin + (int)blockIdx.x;
   const int k = a.topk;
   int32_t* ids = a.out + (int64_t)t * k;
-  const RowPos r = locate(a, p, t);
-  const int n = r.b < 0 ? 0 : r.thr;
-  const int32_t* table = r.b < 0 ? nullptr : a.block_table + (int64_t)r.b * a.table_len;
 
   // Ids of the rows that `taken` says, in order: each wave owns a run of the row, counts what it
   // takes, and writes behind the waves before it. Of the rows that `tied` says the first
@@ -627,37 +765,10 @@ __global__ __launch_bounds__(THREADS) void select_kernel(SasSelectArgs a, SelPla
     for (int i = all + tid; i < k; i += THREADS) ids[i] = -1;
   };
 
-  if (n <= k) {
-    auto there = [&](int j) {
-      const int page = table[p.page_div.div(j)];
-      return page >= 0 && page < a.block_num;
-    };
-    emit(there, [](int) { return false; }, 0);
-    return;
-  }
-
-  // the bound on a score's error
-  float* g = p.score + (int64_t)(t - p.t_begin) * p.width;
-  float kn = 0.0f;
-  {
-    const int thr_end = thr_at(a, p, min(r.last, p.t_end) - 1);
-    const int parts = (thr_end + p.chunk - 1) / p.chunk * p.slices;
-    const float* kp = p.k_norm + (int64_t)r.b * p.chunks * p.slices;
-    for (int i = lane; i < parts; i += 64) kn = max_nonneg(kn, kp[i]);
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) kn = max_nonneg(kn, __shfl_xor(kn, off, 64));
-  }
-  const float wn = p.w_norm[t - p.t_begin];
-  float err = (float)(a.dim + a.heads + 4) * 1.1920929e-7f * wn * (sqrtf(kn) + SEL_TINY);
-  if (kn == 0.0f || wn == 0.0f) err = 0.0f;  // every score is exactly 0
-  if (!(err <= SEL_MAX)) err = __builtin_inff();
-
-  // the row into LDS where it fits, its range, and how many rows there are to choose from
   float lo = SEL_MAX, hi = -SEL_MAX;
   int there = 0, edge = 0;
   for (int j = tid; j < n; j += THREADS) {
-    const float x = g[j];
-    if (ROWCAP > 0) sh.row[j] = x;
+    const float x = x_of[j];
     if (x != SEL_NONE) {
       lo = fminf(lo, x);
       hi = fmaxf(hi, x);
@@ -665,23 +776,9 @@ __global__ __launch_bounds__(THREADS) void select_kernel(SasSelectArgs a, SelPla
       edge |= fabsf(x) >= SEL_MAX;
     }
   }
-  float* x_of = ROWCAP > 0 ? sh.row : g;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    lo = fminf(lo, __shfl_xor(lo, off, 64));
-    hi = fmaxf(hi, __shfl_xor(hi, off, 64));
-  }
-  if (lane == 0) {
-    sh.wave_lo[wave] = lo;
-    sh.wave_hi[wave] = hi;
-  }
+  block_range<THREADS>(lo, hi, sh);
   there = block_sum<THREADS>(there, sh.wave_a);
   edge = block_sum<THREADS>(edge, sh.wave_b);
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    lo = fminf(lo, sh.wave_lo[w]);
-    hi = fmaxf(hi, sh.wave_hi[w]);
-  }
   if (edge) err = __builtin_inff();
   if (there <= k) {
     emit([&](int j) { return x_of[j] != SEL_NONE; }, [](int) { return false; }, 0);
@@ -692,11 +789,11 @@ __global__ __launch_bounds__(THREADS) void select_kernel(SasSelectArgs a, SelPla
   // that holds it, until it is known or the range cannot be cut any more
   int need = k;
   while (lo < hi) {
-    const float base = 0.5f * lo, inv = (float)(SEL_BINS - 1) / (0.5f * hi - base);
-    if (!(inv < SEL_MAX)) break;
-    auto bin_of = [&](float x) { return min((int)((0.5f * x - base) * inv), SEL_BINS - 1); };
+    const BinMap<THREADS> map = BinMap<THREADS>::of(lo, hi);
+    if (!map.usable()) break;
+    auto bin_of = [&](float x) { return max(map.bin(x), 0); };
     __syncthreads();
-    for (int i = tid; i < SEL_BINS; i += THREADS) sh.bins[i] = 0;
+    for (int i = tid; i < BINS; i += THREADS) sh.bins[i] = 0;
     if (tid == 0) sh.count = 0;
     __syncthreads();
     for (int j = tid; j < n; j += THREADS) {
@@ -704,38 +801,10 @@ __global__ __launch_bounds__(THREADS) void select_kernel(SasSelectArgs a, SelPla
       if (x >= lo && x <= hi) atomicAdd(&sh.bins[bin_of(x)], 1u);
     }
     __syncthreads();
-    // counts from the top: thread i owns bins [top - (i + 1) PER, top - i PER)
-    constexpr int PER = SEL_BINS / THREADS;
-    uint32_t c[PER];
-    int sum = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      c[i] = sh.bins[SEL_BINS - 1 - (tid * PER + i)];
-      sum += (int)c[i];
-    }
-    int incl = sum;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int v = __shfl_up(incl, off, 64);
-      if (lane >= off) incl += v;
-    }
-    if (lane == 63) sh.wave_a[wave] = incl;
-    __syncthreads();
-    int before = incl - sum;
-    for (int w = 0; w < wave; ++w) before += sh.wave_a[w];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      if (before < need && need <= before + (int)c[i]) {
-        sh.found = SEL_BINS - 1 - (tid * PER + i);
-        sh.below = before;
-        sh.in_bin = (int)c[i];
-      }
-      before += (int)c[i];
-    }
-    __syncthreads();
+    find_bin<THREADS>(need, sh);
     const int bin = sh.found, in_bin = sh.in_bin;
     need -= sh.below;
-    if (in_bin <= SEL_LIST) {
+    if (in_bin <= LIST) {
       for (int j = tid; j < n; j += THREADS) {
         const float x = x_of[j];
         if (x >= lo && x <= hi && bin_of(x) == bin) sh.list_x[atomicAdd(&sh.count, 1)] = x;
@@ -762,21 +831,7 @@ __global__ __launch_bounds__(THREADS) void select_kernel(SasSelectArgs a, SelPla
         h2 = fmaxf(h2, x);
       }
     }
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      l2 = fminf(l2, __shfl_xor(l2, off, 64));
-      h2 = fmaxf(h2, __shfl_xor(h2, off, 64));
-    }
-    if (lane == 0) {
-      sh.wave_lo[wave] = l2;
-      sh.wave_hi[wave] = h2;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      l2 = fminf(l2, sh.wave_lo[w]);
-      h2 = fmaxf(h2, sh.wave_hi[w]);
-    }
+    block_range<THREADS>(l2, h2, sh);
     if (l2 == lo && h2 == hi) break;
     lo = l2;
     hi = h2;
@@ -794,7 +849,7 @@ __global__ __launch_bounds__(THREADS) void select_kernel(SasSelectArgs a, SelPla
     sure += x > b_hi;
     if (x >= b_lo && x <= b_hi && x != SEL_NONE) {
       const int i = atomicAdd(&sh.count, 1);
-      if (i < SEL_LIST) sh.list_j[i] = j;
+      if (i < LIST) sh.list_j[i] = j;
     }
   }
   sure = block_sum<THREADS>(sure, sh.wave_a);
@@ -808,10 +863,11 @@ __global__ __launch_bounds__(THREADS) void select_kernel(SasSelectArgs a, SelPla
     return;
   }
   const float taken_x = __builtin_inff();
-  if (close <= SEL_LIST) {
-    for (int i = wave; i < close; i += WAVES) {
-      const double s = score64<T, FP8>(a, p, t, table, sh.list_j[i], lane);
-      if (lane == 0) sh.list_key[i] = order_of(s);
+  if (close <= LIST) {
+    for (int i = 16 * wave; i < close; i += 16 * WAVES) {
+      const int e = min(i + (lane & 15), close - 1);
+      const uint64_t key = order64<T, FP8>(a, p, t, table, sh.list_j[e], lane);
+      if (lane < 16 && i + lane < close) sh.list_key[i + lane] = key;
     }
     __syncthreads();
     for (int i = tid; i < close; i += THREADS) {
@@ -836,11 +892,13 @@ __global__ __launch_bounds__(THREADS) void select_kernel(SasSelectArgs a, SelPla
   for (int shift = 56; shift >= 0; shift -= 8) {
     for (int i = tid; i < 256; i += THREADS) sh.bins[i] = 0;
     __syncthreads();
-    for (int j = wave; j < n; j += WAVES) {
+    for (int j0 = 16 * wave; j0 < n; j0 += 16 * WAVES) {
+      const int j = min(j0 + (lane & 15), n - 1);
       const float x = x_of[j];
-      if (!(x >= b_lo && x <= b_hi) || x == SEL_NONE) continue;
-      const uint64_t key = order_of(score64<T, FP8>(a, p, t, table, j, lane));
-      if (lane == 0 && (shift == 56 || key >> (shift + 8) == prefix))
+      const bool in = x >= b_lo && x <= b_hi && x != SEL_NONE && j0 + (lane & 15) < n;
+      if (!__any(in)) continue;
+      const uint64_t key = order64<T, FP8>(a, p, t, table, j, lane);
+      if (lane < 16 && in && (shift == 56 || key >> (shift + 8) == prefix))
         atomicAdd(&sh.bins[(key >> shift) & 255], 1u);
     }
     __syncthreads();
@@ -850,17 +908,350 @@ __global__ __launch_bounds__(THREADS) void select_kernel(SasSelectArgs a, SelPla
     prefix = (prefix << 8) | (uint64_t)digit;
     __syncthreads();
   }
-  for (int j = wave; j < n; j += WAVES) {
+  for (int j0 = 16 * wave; j0 < n; j0 += 16 * WAVES) {
+    const int j = min(j0 + (lane & 15), n - 1);
     const float x = x_of[j];
     float y = x > b_hi ? taken_x : SEL_NONE;
-    if (x >= b_lo && x <= b_hi && x != SEL_NONE) {
-      const uint64_t key = order_of(score64<T, FP8>(a, p, t, table, j, lane));
-      y = key > prefix ? taken_x : key == prefix ? SEL_MAX : SEL_NONE;
+    const bool in = x >= b_lo && x <= b_hi && x != SEL_NONE;
+    if (__any(in)) {
+      const uint64_t key = order64<T, FP8>(a, p, t, table, j, lane);
+      if (in) y = key > prefix ? taken_x : key == prefix ? SEL_MAX : SEL_NONE;
     }
-    if (lane == 0) x_of[j] = y;
+    if (lane < 16 && j0 + lane < n) x_of[j] = y;
   }
   __syncthreads();
   emit([&](int j) { return x_of[j] > SEL_MAX; }, [&](int j) { return x_of[j] == SEL_MAX; }, want);
+}
+
+// Rows longer than this have no place in the map of select_kernel's ids.
+constexpr int SEL_SAMPLED_KEYS = 1 << 18;
+
+// Scores a thread owns of a row of n: the fewest, in whole 16 bytes.
+__device__ inline int listed_width(int n, int threads, int most) {
+  return min(((n + threads - 1) / threads + 3) & ~3, most);
+}
+
+// SAMPLED: rows of any length, of which at most CAP scores get into registers; else rows of at
+// most CAP. A thread owns VPT scores: neighbours in the row, or in the list of a long one.
+template <typename T, bool FP8, int THREADS, int VPT, bool SAMPLED>
+__global__ __launch_bounds__(THREADS) void select_kernel(SasSelectArgs a, SelPlan p) {
+  constexpr int WAVES = THREADS / 64, BINS = SelSize<THREADS>::BINS, LIST = SelSize<THREADS>::LIST;
+  constexpr int CAP = THREADS * VPT, MAP = SAMPLED ? SEL_SAMPLED_KEYS / 32 : CAP / 32;
+  struct Listed {
+    float x[SAMPLED ? CAP : 1];
+    int id[SAMPLED ? CAP : 1];
+  };
+  __shared__ SelShared<THREADS> sh;
+  __shared__ uint32_t map[MAP];
+  __shared__ union {  // (the list is in registers before any key is scored again)
+    Listed listed;
+    double part[SelSize<THREADS>::PARTS][THREADS == 64 ? 1 : LIST];  // 64-bit scores by 16 heads
+  } u;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int t = p.t_begin + (int)blockIdx.x;
+  const int k = a.topk;
+  int32_t* ids = a.out + (int64_t)t * k;
+  const RowPos r = locate(a, p, t);
+  const int n = r.b < 0 ? 0 : r.thr;
+  const int32_t* table = r.b < 0 ? nullptr : a.block_table + (int64_t)r.b * a.table_len;
+  float* g = p.score + (int64_t)(t - p.t_begin) * p.width;
+
+  if (n <= k) {  // every row there is
+    int at = 0;
+    for (int j0 = 0; j0 < n; j0 += THREADS) {
+      const int j = j0 + tid;
+      bool there = false;
+      if (j < n) {
+        const int page = table[p.page_div.div(j)];
+        there = page >= 0 && page < a.block_num;
+      }
+      int all;
+      const int pos = at + block_before<THREADS>(there, sh.wave_a, all);
+      if (there) ids[pos] = j;
+      at += all;
+    }
+    for (int i = at + tid; i < k; i += THREADS) ids[i] = -1;
+    return;
+  }
+
+  float err = 0.0f;  // the bound on a score's error
+  auto from_registers = [&]() -> bool {
+  // the row, or what of it is above the sample's threshold
+  float x[VPT];
+  int id[SAMPLED ? VPT : 1];
+  int first_id = 0;     // !SAMPLED, or a short row: id of x[0], the others follow
+  bool listed = false;  // the values are u.listed's
+  const int vpt = listed_width(n, THREADS, VPT);
+  float kn = 0.0f;
+  {
+    const int thr_end = thr_at(a, p, min(r.last, p.t_end) - 1), keys = piece_keys(p, thr_end);
+    const int parts = (thr_end + keys - 1) / keys * p.slices;
+    const float* kp = p.k_norm + (int64_t)r.b * p.chunks * p.slices;
+    for (int i = lane; i < parts; i += 64) kn = max_nonneg(kn, kp[i]);
+  }
+  const float wn = p.w_norm[t - p.t_begin];
+  if (!SAMPLED || n <= CAP) {
+    first_id = tid * vpt;
+#pragma unroll
+    for (int i = 0; i < VPT; i += 4) {
+      float4 v = make_float4(SEL_NONE, SEL_NONE, SEL_NONE, SEL_NONE);
+      const int j = first_id + i;
+      if (i < vpt && j < n) {
+        v = *(const float4*)(g + j);
+        if (j + 1 >= n) v.y = SEL_NONE;
+        if (j + 2 >= n) v.z = SEL_NONE;
+        if (j + 3 >= n) v.w = SEL_NONE;
+      }
+      x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
+    }
+  }
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) kn = max_nonneg(kn, __shfl_xor(kn, off, 64));
+  err = (float)(a.dim + a.heads + 4) * 1.1920929e-7f * wn * (sqrtf(kn) + SEL_TINY);
+  if (kn == 0.0f || wn == 0.0f) err = 0.0f;  // every score is exactly 0
+  if (!(err <= SEL_MAX)) err = __builtin_inff();
+  if (err == __builtin_inff()) {
+    return false;
+  }
+
+  BinMap<THREADS> list_map = {0.0f, 0.0f};
+  int list_bin = 0;
+  if (SAMPLED && n > CAP) {
+    // 4 THREADS scores in runs of four, evenly over the row; the list takes what is at or above
+    // the bin of their r-th largest, r a little over topk's share: 6 deviations of a sample of
+    // half as many independent ones
+    float4 v = *(const float4*)(g + 4 * (int)((int64_t)tid * (n / 4) / THREADS));
+    const float s[4] = {v.x, v.y, v.z, v.w};
+    float lo = SEL_MAX, hi = -SEL_MAX;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (s[i] != SEL_NONE) lo = fminf(lo, s[i]), hi = fmaxf(hi, s[i]);
+    }
+    block_range<THREADS>(lo, hi, sh);
+    const float share = (float)k * (4.0f * THREADS) / (float)n;
+    const int want = (int)(share + 6.0f * sqrtf(2.0f * share) + 8.0f);
+    list_map = BinMap<THREADS>::of(lo, hi);
+    if (n > SEL_SAMPLED_KEYS || (float)want * (float)n > 0.85f * CAP * (4.0f * THREADS) || !(lo < hi) ||
+        !list_map.usable()) {
+      return false;
+    }
+    for (int i = tid; i < BINS; i += THREADS) sh.bins[i] = 0;
+    if (tid == 0) {
+      sh.count = 0;
+      sh.found = 0;  // (fewer than `want` rows there in the sample: every row there is)
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (s[i] != SEL_NONE) atomicAdd(&sh.bins[list_map.bin(s[i])], 1u);
+    }
+    __syncthreads();
+    find_bin<THREADS>(want, sh);
+    list_bin = sh.found;
+    auto add = [&](float y, int j) {
+      const bool in = y != SEL_NONE && list_map.bin(y) >= list_bin;
+      const uint64_t m = __ballot(in);
+      if (m == 0) return;
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&sh.count, __popcll(m));
+      at = __builtin_amdgcn_readfirstlane(at) + (int)__popcll(m & (((uint64_t)1 << lane) - 1));
+      if (in && at < CAP) {
+        u.listed.x[at] = y;
+        u.listed.id[at] = j;
+      }
+    };
+    for (int j0 = 0; j0 < n; j0 += 16 * THREADS) {
+      float4 y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = j0 + 4 * (tid + i * THREADS);
+        y[i] = j < n ? *(const float4*)(g + j) : make_float4(SEL_NONE, SEL_NONE, SEL_NONE, SEL_NONE);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = j0 + 4 * (tid + i * THREADS);
+        add(y[i].x, j);
+        add(j + 1 < n ? y[i].y : SEL_NONE, j + 1);
+        add(j + 2 < n ? y[i].z : SEL_NONE, j + 2);
+        add(j + 3 < n ? y[i].w : SEL_NONE, j + 3);
+      }
+    }
+    __syncthreads();
+    const int all = sh.count;
+    if (all > CAP || all < k) {
+      return false;
+    }
+    listed = true;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int e = tid + i * THREADS;
+      x[i] = e < all ? u.listed.x[e] : SEL_NONE;
+      if (SAMPLED) id[i] = e < all ? u.listed.id[e] : 0;
+    }
+  }
+  auto id_of = [&](int i) { return SAMPLED && listed ? id[i] : first_id + i; };
+
+  // 1. the topk-th largest, or a range [lo, hi] around it
+  float lo = SEL_MAX, hi = -SEL_MAX;
+  int there = 0, edge = 0;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    if (x[i] != SEL_NONE) {
+      lo = fminf(lo, x[i]);
+      hi = fmaxf(hi, x[i]);
+      ++there;
+      edge |= fabsf(x[i]) >= SEL_MAX;
+    }
+  }
+  const int map_words = (n + 31) / 32;
+  for (int i = tid; i < map_words; i += THREADS) map[i] = 0;
+  for (int i = tid; i < BINS; i += THREADS) sh.bins[i] = 0;
+  block_range<THREADS>(lo, hi, sh);  // (a barrier: the list's length has been read)
+  if (tid == 0) sh.count = 0;
+  there = block_sum<THREADS>(there | (edge << 16), sh.wave_a);
+  __syncthreads();
+  auto take = [&](int j) { atomicOr(&map[j >> 5], 1u << (j & 31)); };
+  if (there >> 16) {
+    err = __builtin_inff();
+    return false;
+  }
+  if (there <= k) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      if (x[i] != SEL_NONE) take(id_of(i));
+    }
+  } else {
+    const BinMap<THREADS> m = BinMap<THREADS>::of(lo, hi);
+    if (!(lo < hi) || !m.usable() || err == 0.0f) {  // all alike: nothing to rank by
+      return false;
+    }
+    // (of many values per thread only those above a bin that a sample of them puts a little
+    // below the topk-th are counted: 6 deviations, of a sample of half as many independent ones)
+    int floor_bin = 0;
+    if (VPT >= 16 && THREADS == 1024 && vpt >= 16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (x[i] != SEL_NONE) atomicAdd(&sh.bins[m.bin(x[i])], 1u);
+      }
+      if (tid == 0) sh.found = 0;
+      const float share = (float)k * 4.0f / (float)vpt;
+      __syncthreads();
+      find_bin<THREADS>((int)(share + 6.0f * sqrtf(2.0f * share) + 8.0f), sh);
+      floor_bin = sh.found;
+      __syncthreads();
+      for (int i = tid; i < BINS; i += THREADS) sh.bins[i] = 0;
+      __syncthreads();
+    }
+    auto count = [&](int from) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int b = m.bin(x[i]);
+        if (x[i] != SEL_NONE && b >= from && (from == floor_bin || b < floor_bin)) atomicAdd(&sh.bins[b], 1u);
+      }
+      if (tid == 0) sh.found = -1;
+      __syncthreads();
+      find_bin<THREADS>(k, sh);
+    };
+    count(floor_bin);
+    if (floor_bin > 0 && sh.found < 0) {  // (the sample put it too high: the others are counted too)
+      __syncthreads();
+      count(0);
+    }
+    const int bin = sh.found, in_bin = sh.in_bin, need = k - sh.below;
+    if (in_bin > LIST) {
+      return false;
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      if (x[i] != SEL_NONE && m.bin(x[i]) == bin) sh.list_x[atomicAdd(&sh.count, 1)] = x[i];
+    }
+    __syncthreads();
+    for (int i = tid; i < in_bin; i += THREADS) {
+      const float y = sh.list_x[i];
+      int above = 0, same = 0;
+      for (int e = 0; e < in_bin; ++e) {
+        above += sh.list_x[e] > y;
+        same += sh.list_x[e] == y;
+      }
+      if (above < need && need <= above + same) sh.value = y;
+    }
+    __syncthreads();
+    const float kth = sh.value;
+
+    // 2. rows within the bound of it
+    const float b_lo = kth - 2.0f * err, b_hi = kth + 2.0f * err;
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    int sure = 0;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      sure += x[i] > b_hi;
+      if (x[i] >= b_lo && x[i] <= b_hi && x[i] != SEL_NONE) {
+        const int e = atomicAdd(&sh.count, 1);
+        if (e < LIST) sh.list_j[e] = id_of(i);
+      }
+    }
+    sure = block_sum<THREADS>(sure, sh.wave_b);
+    __syncthreads();
+    const int close = sh.count, rest = k - sure;  // `rest` of the `close` rows are taken
+    if (close > LIST || (SAMPLED && listed && list_map.bin(b_lo) < list_bin)) {
+      return false;
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      if (x[i] > b_hi) take(id_of(i));
+    }
+    if (close == rest) {
+      for (int i = tid; i < close; i += THREADS) take(sh.list_j[i]);
+    } else {
+      const int groups = (close + 15) / 16, heads16 = (a.heads + 15) / 16;
+      if (WAVES == 1) {
+        for (int i = 0; i < close; i += 16) {
+          const uint64_t key = order64<T, FP8>(a, p, t, table, sh.list_j[min(i + (lane & 15), close - 1)], lane);
+          if (lane < 16 && i + lane < close) sh.list_key[i + lane] = key;
+        }
+      } else {
+        for (int i = wave; i < groups * heads16; i += WAVES) {
+          const int e = i / heads16 * 16, h16 = i % heads16;
+          const double s = score64_part<T, FP8>(a, p, t, table, sh.list_j[min(e + (lane & 15), close - 1)],
+                                                16 * h16, lane);
+          if (lane < 16 && e + lane < close) u.part[h16][e + lane] = s;
+        }
+        __syncthreads();
+        for (int i = tid; i < close; i += THREADS) {
+          double s = 0.0;
+          for (int h16 = 0; h16 < heads16; ++h16) s += u.part[h16][i];
+          sh.list_key[i] = order_of(s * key_scale64<FP8>(a, p, table, sh.list_j[i]));
+        }
+      }
+      __syncthreads();
+      for (int i = tid; i < close; i += THREADS) {
+        const uint64_t key = sh.list_key[i];
+        const int j = sh.list_j[i];
+        int rank = 0;
+        for (int e = 0; e < close; ++e) {
+          const uint64_t o = sh.list_key[e];
+          rank += o > key || (o == key && sh.list_j[e] < j);
+        }
+        if (rank < rest) take(j);
+      }
+    }
+  }
+  __syncthreads();
+
+  // 3. the ids in order
+  const int per = (map_words + THREADS - 1) / THREADS, w0 = min(tid * per, map_words),
+            w1 = min(w0 + per, map_words);
+  int mine = 0, all;
+  for (int w = w0; w < w1; ++w) mine += __popc(map[w]);
+  int pos = block_before<THREADS>(mine, sh.wave_a, all);
+  for (int w = w0; w < w1; ++w) {
+    for (uint32_t bits = map[w]; bits; bits &= bits - 1) ids[pos++] = 32 * w + __builtin_ctz(bits);
+  }
+  for (int i = all + tid; i < k; i += THREADS) ids[i] = -1;
+  return true;
+  };
+  if (!from_registers()) select_from_memory<T, FP8, THREADS>(a, p, t, n, err, g, table, sh);
 }
 
 // ---------------------------------------------------------------------------
@@ -890,15 +1281,10 @@ PassPlan plan_passes(const SasSelectArgs& a) {
   p.wq = r.tiles ? TILE_WAVES : per_seq >= 2 ? 2 : 1;
   p.slices = r.tiles ? 1 : 4 / p.wq;
   const int64_t groups = (r.rows + p.wq - 1) / p.wq;
-  if (r.tiles) {
-    p.chunk = 512;
-  } else {
-    int64_t c = (int64_t)p.width * groups / 2048;
-    const int unit = 64 * p.slices;
-    c = (c + unit - 1) / unit * unit;
-    p.chunk = (int)(c < unit ? unit : c > 2048 ? 2048 : c);
-  }
-  p.chunks = (p.width + p.chunk - 1) / p.chunk;
+  // enough workgroups to fill the chip a few times over, of at least 64 keys a slice
+  const int64_t most = (p.width + 64 * p.slices - 1) / (64 * p.slices);
+  const int64_t pieces = ((r.tiles ? 512 : 1024) + groups - 1) / (groups < 1 ? 1 : groups);
+  p.chunks = (int)(pieces < 1 ? 1 : pieces > most ? most : pieces);
   // every part starts on 16 bytes
   const int64_t w_floats = ((int64_t)r.rows + 3) / 4 * 4;
   const int64_t k_floats = ((int64_t)a.batch * p.chunks * p.slices + 3) / 4 * 4;
@@ -966,13 +1352,16 @@ void launch_pass(const SasSelectArgs& a, const PassPlan& r, const SelPlan& p, hi
       else launch_scores<T, FP8, 64, 4>(a, r, p, st);
     }
   }
-  const dim3 grid((unsigned)(p.t_end - p.t_begin));
-  if (a.max_keys <= 4096) {
-    hipLaunchKernelGGL((select_kernel<T, FP8, 256, 4096>), grid, dim3(256), 0, st, a, p);
+  const int rows = p.t_end - p.t_begin;
+  const dim3 grid((unsigned)rows);
+  if (a.max_keys <= 2048 && rows >= 512) {
+    hipLaunchKernelGGL((select_kernel<T, FP8, 64, 32, false>), grid, dim3(64), 0, st, a, p);
+  } else if (a.max_keys <= 8192) {
+    hipLaunchKernelGGL((select_kernel<T, FP8, 256, 32, false>), grid, dim3(256), 0, st, a, p);
   } else if (a.max_keys <= 32768) {
-    hipLaunchKernelGGL((select_kernel<T, FP8, 1024, 32768>), grid, dim3(1024), 0, st, a, p);
+    hipLaunchKernelGGL((select_kernel<T, FP8, 1024, 32, false>), grid, dim3(1024), 0, st, a, p);
   } else {
-    hipLaunchKernelGGL((select_kernel<T, FP8, 1024, 0>), grid, dim3(1024), 0, st, a, p);
+    hipLaunchKernelGGL((select_kernel<T, FP8, 1024, 8, true>), grid, dim3(1024), 0, st, a, p);
   }
 }
 
