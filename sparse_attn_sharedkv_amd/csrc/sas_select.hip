@@ -97,6 +97,15 @@ __device__ inline u32x4 widen_e4m3(u32x2 c) {
   return __builtin_bit_cast(u32x4, r);
 }
 
+// The bound on an fp32 score's error: 0 where every score is exactly 0, infinite where it says
+// nothing.
+__device__ inline float score_error(const SasSelectArgs& a, float w_norm, float k_norm2) {
+  const float err = ((float)a.dim + (float)a.heads / 16.0f + 8.0f) * 1.1920929e-7f * w_norm *
+                    (sqrtf(k_norm2) + SEL_TINY);
+  if (k_norm2 == 0.0f || w_norm == 0.0f) return 0.0f;
+  return err <= SEL_MAX ? err : __builtin_inff();
+}
+
 // What both kernels know of a launch besides its arguments.
 struct SelPlan {
   int t_begin, t_end;   // query rows of this pass
@@ -515,9 +524,11 @@ struct SelShared {
   float list_x[S::LIST];
   int list_j[S::LIST];
   uint64_t list_key[S::LIST];
+  int sums[8][S::WAVES];  // by SelSlot
   int wave_a[S::WAVES], wave_b[S::WAVES];
   float wave_lo[S::WAVES], wave_hi[S::WAVES];
-  int count, found, below, in_bin;
+  int close_j[S::LIST];
+  int count, found, below, in_bin, sure, close;
   float value;
 };
 
@@ -610,30 +621,73 @@ __device__ inline uint64_t order64(const SasSelectArgs& a, const SelPlan& p, int
   return order_of(s * key_scale64<FP8>(a, p, table, j));
 }
 
+// Reductions over a wave on the vector ALU (data-parallel shifts; lane 63 ends with the result).
+template <typename F>
+__device__ inline int wave_scan(int v, int identity, F op) {
+  v = op(v, __builtin_amdgcn_update_dpp(identity, v, 0x111, 0xf, 0xf, false));  // row_shr:1
+  v = op(v, __builtin_amdgcn_update_dpp(identity, v, 0x112, 0xf, 0xf, false));
+  v = op(v, __builtin_amdgcn_update_dpp(identity, v, 0x114, 0xf, 0xf, false));
+  v = op(v, __builtin_amdgcn_update_dpp(identity, v, 0x118, 0xf, 0xf, false));
+  v = op(v, __builtin_amdgcn_update_dpp(identity, v, 0x142, 0xa, 0xf, false));  // row_bcast:15
+  return op(v, __builtin_amdgcn_update_dpp(identity, v, 0x143, 0xc, 0xf, false));  // row_bcast:31
+}
+__device__ inline int as_int(float f) { return __builtin_bit_cast(int, f); }
+__device__ inline float as_float(int i) { return __builtin_bit_cast(float, i); }
+__device__ inline int wave_incl(int v) {
+  return wave_scan(v, 0, [](int a, int b) { return a + b; });
+}
+__device__ inline int wave_sum(int v) { return __builtin_amdgcn_readlane(wave_incl(v), 63); }
+__device__ inline float wave_min(float v) {
+  const int r = wave_scan(as_int(v), as_int(SEL_MAX), [](int a, int b) {
+    return as_int(fminf(as_float(a), as_float(b)));
+  });
+  return as_float(__builtin_amdgcn_readlane(r, 63));
+}
+__device__ inline float wave_max(float v) { return -wave_min(-v); }
+
+// The workgroup's sums take one barrier each: every use has a row of sh.sums of its own.
+enum SelSlot { SLOT_THERE, SLOT_SAMPLE, SLOT_COUNT, SLOT_ABOVE, SLOT_IDS, SLOT_FREE, SLOT_NUM };
+
 template <int THREADS>
-__device__ inline int block_sum(int v, int* scratch) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(v, off, 64);
+__device__ inline int block_sum(int v, SelSlot slot, SelShared<THREADS>& sh) {
+  v = wave_sum(v);
   if (THREADS == 64) return v;
+  if ((threadIdx.x & 63) == 0) sh.sums[slot][threadIdx.x >> 6] = v;
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
-  __syncthreads();
-  int s = 0;
+  v = 0;
 #pragma unroll
-  for (int i = 0; i < THREADS / 64; ++i) s += scratch[i];
-  return s;
+  for (int w = 0; w < THREADS / 64; ++w) v += sh.sums[slot][w];
+  return v;
+}
+
+// Sum of the threads' values before this one's; `all` is the sum of every thread's.
+template <int THREADS>
+__device__ inline int block_before(int v, SelSlot slot, SelShared<THREADS>& sh, int& all) {
+  const int incl = wave_incl(v);
+  if (THREADS == 64) {
+    all = __builtin_amdgcn_readlane(incl, 63);
+    return incl - v;
+  }
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 63) sh.sums[slot][wave] = incl;
+  __syncthreads();
+  int before = incl - v;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    before += w < wave ? sh.sums[slot][w] : 0;
+    all += sh.sums[slot][w];
+  }
+  return before;
 }
 
 // The range of the workgroup's values, the same in every thread.
 template <int THREADS>
 __device__ inline void block_range(float& lo, float& hi, SelShared<THREADS>& sh) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    lo = fminf(lo, __shfl_xor(lo, off, 64));
-    hi = fmaxf(hi, __shfl_xor(hi, off, 64));
-  }
+  lo = wave_min(lo);
+  hi = wave_max(hi);
   if (THREADS == 64) return;
-  __syncthreads();
+  __syncthreads();  // (its two rows have several uses)
   if ((threadIdx.x & 63) == 0) {
     sh.wave_lo[threadIdx.x >> 6] = lo;
     sh.wave_hi[threadIdx.x >> 6] = hi;
@@ -646,37 +700,10 @@ __device__ inline void block_range(float& lo, float& hi, SelShared<THREADS>& sh)
   }
 }
 
-// Sum of the threads' values before this one's; `all` is the sum of every thread's.
-template <int THREADS>
-__device__ inline int block_before(int v, int* scratch, int& all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int incl = v;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int u = __shfl_up(incl, off, 64);
-    if (lane >= off) incl += u;
-  }
-  if (THREADS == 64) {
-    all = __shfl(incl, 63, 64);
-    return incl - v;
-  }
-  __syncthreads();
-  if (lane == 63) scratch[wave] = incl;
-  __syncthreads();
-  int before = incl - v;
-  all = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) {
-    before += w < wave ? scratch[w] : 0;
-    all += scratch[w];
-  }
-  return before;
-}
-
 // Finds the bin that holds the need-th value from the top: sh.found, the values above it
 // sh.below, and its own sh.in_bin. Ends with a barrier.
 template <int THREADS>
-__device__ inline void find_bin(int need, SelShared<THREADS>& sh) {
+__device__ inline void find_bin(int need, SelSlot slot, SelShared<THREADS>& sh) {
   constexpr int BINS = SelSize<THREADS>::BINS, PER = BINS / THREADS;
   int c[PER], sum = 0, all;
 #pragma unroll
@@ -684,7 +711,7 @@ __device__ inline void find_bin(int need, SelShared<THREADS>& sh) {
     c[i] = (int)sh.bins[BINS - 1 - ((int)threadIdx.x * PER + i)];
     sum += c[i];
   }
-  int before = block_before<THREADS>(sum, sh.wave_a, all);
+  int before = block_before<THREADS>(sum, slot, sh, all);
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     if (before < need && need <= before + c[i]) {
@@ -705,6 +732,7 @@ struct BinMap {
     return {0.5f * lo, (float)(SelSize<THREADS>::BINS - 1) / (0.5f * hi - 0.5f * lo)};
   }
   __device__ bool usable() const { return inv < SEL_MAX; }
+  __device__ float edge(int bin) const { return 2.0f * ((float)bin / inv + base); }  // about
   __device__ int bin(float x) const {
     const float b = fminf((0.5f * x - base) * inv, (float)(SelSize<THREADS>::BINS - 1));
     return b < 0.0f ? -1 : (int)b;
@@ -777,8 +805,9 @@ __device__ inline void select_from_memory(const SasSelectArgs& a, const SelPlan&
     }
   }
   block_range<THREADS>(lo, hi, sh);
-  there = block_sum<THREADS>(there, sh.wave_a);
-  edge = block_sum<THREADS>(edge, sh.wave_b);
+  __syncthreads();
+  there = block_sum<THREADS>(there, SLOT_THERE, sh);
+  edge = block_sum<THREADS>(edge, SLOT_ABOVE, sh);
   if (edge) err = __builtin_inff();
   if (there <= k) {
     emit([&](int j) { return x_of[j] != SEL_NONE; }, [](int) { return false; }, 0);
@@ -801,7 +830,7 @@ __device__ inline void select_from_memory(const SasSelectArgs& a, const SelPlan&
       if (x >= lo && x <= hi) atomicAdd(&sh.bins[bin_of(x)], 1u);
     }
     __syncthreads();
-    find_bin<THREADS>(need, sh);
+    find_bin<THREADS>(need, SLOT_COUNT, sh);
     const int bin = sh.found, in_bin = sh.in_bin;
     need -= sh.below;
     if (in_bin <= LIST) {
@@ -852,7 +881,8 @@ __device__ inline void select_from_memory(const SasSelectArgs& a, const SelPlan&
       if (i < LIST) sh.list_j[i] = j;
     }
   }
-  sure = block_sum<THREADS>(sure, sh.wave_a);
+  sure = block_sum<THREADS>(sure, SLOT_SAMPLE, sh);
+  __syncthreads();
   const int close = sh.count, rest = k - sure;  // `rest` of the `close` rows are taken
   if (exact) {
     emit([&](int j) { return x_of[j] > hi; }, [&](int j) { return x_of[j] == hi; }, rest);
@@ -926,15 +956,37 @@ __device__ inline void select_from_memory(const SasSelectArgs& a, const SelPlan&
 // Rows longer than this have no place in the map of select_kernel's ids.
 constexpr int SEL_SAMPLED_KEYS = 1 << 18;
 
-// Scores a thread owns of a row of n: the fewest, in whole 16 bytes.
-__device__ inline int listed_width(int n, int threads, int most) {
-  return min(((n + threads - 1) / threads + 3) & ~3, most);
+// Eight bits to every fourth bit.
+__device__ inline uint32_t every_fourth(uint32_t b) {
+  b = (b | (b << 12)) & 0x000f000fu;
+  b = (b | (b << 6)) & 0x03030303u;
+  return (b | (b << 3)) & 0x11111111u;
+}
+
+// Where the rank of `count` listed values (larger first, equal ones by id) is `want`, says so.
+template <int THREADS, typename K, typename F>
+__device__ inline void rank_list(int count, const K* key, const int* id, F at) {
+  constexpr int SHARE = THREADS == 64 ? 1 : 16;  // lanes that rank one value
+  for (int i = threadIdx.x / SHARE; i < count; i += THREADS / SHARE) {
+    const K x = key[i];
+    const int j = id[i];
+    int rank = 0;
+#pragma unroll 4
+    for (int e = threadIdx.x % SHARE; e < count; e += SHARE) {
+      const K y = key[e];
+      rank += y > x || (y == x && id[e] < j);
+    }
+#pragma unroll
+    for (int off = 1; off < SHARE; off <<= 1) rank += __shfl_xor(rank, off, 64);
+    if (threadIdx.x % SHARE == 0) at(i, rank);
+  }
 }
 
 // SAMPLED: rows of any length, of which at most CAP scores get into registers; else rows of at
-// most CAP. A thread owns VPT scores: neighbours in the row, or in the list of a long one.
+// most CAP. Value i of a thread is id (i / 4) 4 THREADS + 4 tid + i % 4 (whole 16 bytes, side by
+// side in a wave), or what the list of a long row has.
 template <typename T, bool FP8, int THREADS, int VPT, bool SAMPLED>
-__global__ __launch_bounds__(THREADS) void select_kernel(SasSelectArgs a, SelPlan p) {
+__global__ __launch_bounds__(THREADS, THREADS == 64 ? 5 : 4) void select_kernel(SasSelectArgs a, SelPlan p) {
   constexpr int WAVES = THREADS / 64, BINS = SelSize<THREADS>::BINS, LIST = SelSize<THREADS>::LIST;
   constexpr int CAP = THREADS * VPT, MAP = SAMPLED ? SEL_SAMPLED_KEYS / 32 : CAP / 32;
   struct Listed {
@@ -942,7 +994,9 @@ __global__ __launch_bounds__(THREADS) void select_kernel(SasSelectArgs a, SelPla
     int id[SAMPLED ? CAP : 1];
   };
   __shared__ SelShared<THREADS> sh;
-  __shared__ uint32_t map[MAP];
+  // taken ids. A listed row: id j is bit j. Else in the order the waves vote: a run of 256 ids has
+  // four numbers of 64 bits, bit l of number c is the run's id 4 l + c
+  __shared__ __attribute__((aligned(16))) uint32_t map[MAP];
   __shared__ union {  // (the list is in registers before any key is scored again)
     Listed listed;
     double part[SelSize<THREADS>::PARTS][THREADS == 64 ? 1 : LIST];  // 64-bit scores by 16 heads
@@ -966,9 +1020,10 @@ __global__ __launch_bounds__(THREADS) void select_kernel(SasSelectArgs a, SelPla
         there = page >= 0 && page < a.block_num;
       }
       int all;
-      const int pos = at + block_before<THREADS>(there, sh.wave_a, all);
+      const int pos = at + block_before<THREADS>(there, SLOT_IDS, sh, all);
       if (there) ids[pos] = j;
       at += all;
+      __syncthreads();
     }
     for (int i = at + tid; i < k; i += THREADS) ids[i] = -1;
     return;
@@ -976,282 +1031,311 @@ __global__ __launch_bounds__(THREADS) void select_kernel(SasSelectArgs a, SelPla
 
   float err = 0.0f;  // the bound on a score's error
   auto from_registers = [&]() -> bool {
-  // the row, or what of it is above the sample's threshold
-  float x[VPT];
-  int id[SAMPLED ? VPT : 1];
-  int first_id = 0;     // !SAMPLED, or a short row: id of x[0], the others follow
-  bool listed = false;  // the values are u.listed's
-  const int vpt = listed_width(n, THREADS, VPT);
-  float kn = 0.0f;
-  {
-    const int thr_end = thr_at(a, p, min(r.last, p.t_end) - 1), keys = piece_keys(p, thr_end);
-    const int parts = (thr_end + keys - 1) / keys * p.slices;
-    const float* kp = p.k_norm + (int64_t)r.b * p.chunks * p.slices;
-    for (int i = lane; i < parts; i += 64) kn = max_nonneg(kn, kp[i]);
-  }
-  const float wn = p.w_norm[t - p.t_begin];
-  if (!SAMPLED || n <= CAP) {
-    first_id = tid * vpt;
+    float x[VPT];
+    int id[SAMPLED ? VPT : 1];
+    const bool listed = SAMPLED && n > CAP;
+    auto none = [] { return make_float4(SEL_NONE, SEL_NONE, SEL_NONE, SEL_NONE); };
+    auto load4 = [&](int j) {
+      float4 v = none();
+      if (j < n) v = *(const float4*)(g + j);
+      if (j + 1 >= n) v.y = SEL_NONE;
+      if (j + 2 >= n) v.z = SEL_NONE;
+      if (j + 3 >= n) v.w = SEL_NONE;
+      return v;
+    };
+    const int runs = (n + 4 * THREADS - 1) / (4 * THREADS);  // of !listed values
+    float4 sample = none();
+    if (listed) {
+      sample = *(const float4*)(g + 4 * (int)((int64_t)tid * (n / 4) / THREADS));
+    } else {
 #pragma unroll
-    for (int i = 0; i < VPT; i += 4) {
-      float4 v = make_float4(SEL_NONE, SEL_NONE, SEL_NONE, SEL_NONE);
-      const int j = first_id + i;
-      if (i < vpt && j < n) {
-        v = *(const float4*)(g + j);
-        if (j + 1 >= n) v.y = SEL_NONE;
-        if (j + 2 >= n) v.z = SEL_NONE;
-        if (j + 3 >= n) v.w = SEL_NONE;
+      for (int i = 0; i < VPT; i += 4) {
+        const float4 v = i / 4 < runs ? load4(i * THREADS + 4 * tid) : none();
+        x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
       }
-      x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
     }
-  }
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) kn = max_nonneg(kn, __shfl_xor(kn, off, 64));
-  err = (float)(a.dim + a.heads + 4) * 1.1920929e-7f * wn * (sqrtf(kn) + SEL_TINY);
-  if (kn == 0.0f || wn == 0.0f) err = 0.0f;  // every score is exactly 0
-  if (!(err <= SEL_MAX)) err = __builtin_inff();
-  if (err == __builtin_inff()) {
-    return false;
-  }
-
-  BinMap<THREADS> list_map = {0.0f, 0.0f};
-  int list_bin = 0;
-  if (SAMPLED && n > CAP) {
-    // 4 THREADS scores in runs of four, evenly over the row; the list takes what is at or above
-    // the bin of their r-th largest, r a little over topk's share: 6 deviations of a sample of
-    // half as many independent ones
-    float4 v = *(const float4*)(g + 4 * (int)((int64_t)tid * (n / 4) / THREADS));
-    const float s[4] = {v.x, v.y, v.z, v.w};
-    float lo = SEL_MAX, hi = -SEL_MAX;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (s[i] != SEL_NONE) lo = fminf(lo, s[i]), hi = fmaxf(hi, s[i]);
+    float kn = 0.0f;
+    {
+      const int thr_end = thr_at(a, p, min(r.last, p.t_end) - 1), keys = piece_keys(p, thr_end);
+      const int parts = (thr_end + keys - 1) / keys * p.slices;
+      const float* kp = p.k_norm + (int64_t)r.b * p.chunks * p.slices;
+      for (int i = lane; i < parts; i += 64) kn = max_nonneg(kn, kp[i]);
+      kn = as_float(__builtin_amdgcn_readlane(
+          wave_scan(as_int(kn), 0, [](int a, int b) { return max(a, b); }), 63));
     }
-    block_range<THREADS>(lo, hi, sh);
-    const float share = (float)k * (4.0f * THREADS) / (float)n;
-    const int want = (int)(share + 6.0f * sqrtf(2.0f * share) + 8.0f);
-    list_map = BinMap<THREADS>::of(lo, hi);
-    if (n > SEL_SAMPLED_KEYS || (float)want * (float)n > 0.85f * CAP * (4.0f * THREADS) || !(lo < hi) ||
-        !list_map.usable()) {
-      return false;
-    }
+    const float wn = p.w_norm[t - p.t_begin];
+    err = score_error(a, wn, kn);
+    if (!(err > 0.0f) || err == __builtin_inff()) return false;
     for (int i = tid; i < BINS; i += THREADS) sh.bins[i] = 0;
     if (tid == 0) {
       sh.count = 0;
-      sh.found = 0;  // (fewer than `want` rows there in the sample: every row there is)
+      sh.found = 0;
     }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (s[i] != SEL_NONE) atomicAdd(&sh.bins[list_map.bin(s[i])], 1u);
-    }
-    __syncthreads();
-    find_bin<THREADS>(want, sh);
-    list_bin = sh.found;
-    auto add = [&](float y, int j) {
-      const bool in = y != SEL_NONE && list_map.bin(y) >= list_bin;
-      const uint64_t m = __ballot(in);
-      if (m == 0) return;
-      int at = 0;
-      if (lane == 0) at = atomicAdd(&sh.count, __popcll(m));
-      at = __builtin_amdgcn_readfirstlane(at) + (int)__popcll(m & (((uint64_t)1 << lane) - 1));
-      if (in && at < CAP) {
-        u.listed.x[at] = y;
-        u.listed.id[at] = j;
-      }
-    };
-    for (int j0 = 0; j0 < n; j0 += 16 * THREADS) {
-      float4 y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = j0 + 4 * (tid + i * THREADS);
-        y[i] = j < n ? *(const float4*)(g + j) : make_float4(SEL_NONE, SEL_NONE, SEL_NONE, SEL_NONE);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = j0 + 4 * (tid + i * THREADS);
-        add(y[i].x, j);
-        add(j + 1 < n ? y[i].y : SEL_NONE, j + 1);
-        add(j + 2 < n ? y[i].z : SEL_NONE, j + 2);
-        add(j + 3 < n ? y[i].w : SEL_NONE, j + 3);
-      }
-    }
-    __syncthreads();
-    const int all = sh.count;
-    if (all > CAP || all < k) {
-      return false;
-    }
-    listed = true;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int e = tid + i * THREADS;
-      x[i] = e < all ? u.listed.x[e] : SEL_NONE;
-      if (SAMPLED) id[i] = e < all ? u.listed.id[e] : 0;
-    }
-  }
-  auto id_of = [&](int i) { return SAMPLED && listed ? id[i] : first_id + i; };
 
-  // 1. the topk-th largest, or a range [lo, hi] around it
-  float lo = SEL_MAX, hi = -SEL_MAX;
-  int there = 0, edge = 0;
+    float floor_x = SEL_NONE;  // listed: every value at or above it is in the list
+    if (listed) {
+      // 4 THREADS scores in runs of four, evenly over the row; the list takes what is at or
+      // above the bin of their want-th largest, a little over topk's share: 6 deviations of a
+      // sample of half as many independent ones
+      const float share = (float)k * (4.0f * THREADS) / (float)n;
+      const int want = (int)(share + 6.0f * sqrtf(2.0f * share) + 8.0f);
+      if (n > SEL_SAMPLED_KEYS || (float)want * (float)n > 0.85f * CAP * (4.0f * THREADS)) return false;
+      auto low = [](float v) { return v != SEL_NONE ? v : SEL_MAX; };
+      float lo = fminf(fminf(low(sample.x), low(sample.y)), fminf(low(sample.z), low(sample.w)));
+      float hi = fmaxf(fmaxf(sample.x, sample.y), fmaxf(sample.z, sample.w));
+      block_range<THREADS>(lo, hi, sh);
+      const BinMap<THREADS> m = BinMap<THREADS>::of(lo, hi);
+      if (!(lo < hi) || !m.usable()) return false;
+      auto tally = [&](float v) {
+        if (v != SEL_NONE) atomicAdd(&sh.bins[m.bin(v)], 1u);
+      };
+      tally(sample.x), tally(sample.y), tally(sample.z), tally(sample.w);
+      __syncthreads();
+      find_bin<THREADS>(want, SLOT_SAMPLE, sh);
+      floor_x = m.edge(sh.found);
+      // (the first bin also takes what the sample has missed below it)
+      if (sh.found == 0) floor_x = -SEL_MAX;
+      // four runs of a thread at a time, the next four on their way
+      float4 y[4], z[4];
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    if (x[i] != SEL_NONE) {
-      lo = fminf(lo, x[i]);
-      hi = fmaxf(hi, x[i]);
-      ++there;
-      edge |= fabsf(x[i]) >= SEL_MAX;
-    }
-  }
-  const int map_words = (n + 31) / 32;
-  for (int i = tid; i < map_words; i += THREADS) map[i] = 0;
-  for (int i = tid; i < BINS; i += THREADS) sh.bins[i] = 0;
-  block_range<THREADS>(lo, hi, sh);  // (a barrier: the list's length has been read)
-  if (tid == 0) sh.count = 0;
-  there = block_sum<THREADS>(there | (edge << 16), sh.wave_a);
-  __syncthreads();
-  auto take = [&](int j) { atomicOr(&map[j >> 5], 1u << (j & 31)); };
-  if (there >> 16) {
-    err = __builtin_inff();
-    return false;
-  }
-  if (there <= k) {
+      for (int i = 0; i < 4; ++i) y[i] = load4(4 * (tid + i * THREADS));
+      for (int j0 = 0; j0 < n; j0 += 16 * THREADS) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      if (x[i] != SEL_NONE) take(id_of(i));
-    }
-  } else {
-    const BinMap<THREADS> m = BinMap<THREADS>::of(lo, hi);
-    if (!(lo < hi) || !m.usable() || err == 0.0f) {  // all alike: nothing to rank by
-      return false;
-    }
-    // (of many values per thread only those above a bin that a sample of them puts a little
-    // below the topk-th are counted: 6 deviations, of a sample of half as many independent ones)
-    int floor_bin = 0;
-    if (VPT >= 16 && THREADS == 1024 && vpt >= 16) {
+        for (int i = 0; i < 4; ++i) z[i] = load4(j0 + 16 * THREADS + 4 * (tid + i * THREADS));
+        int mine = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (x[i] != SEL_NONE) atomicAdd(&sh.bins[m.bin(x[i])], 1u);
+        for (int i = 0; i < 4; ++i)
+          mine += (y[i].x >= floor_x) + (y[i].y >= floor_x) + (y[i].z >= floor_x) + (y[i].w >= floor_x);
+        const int incl = wave_incl(mine);
+        int at = 0;
+        if (lane == 63) at = atomicAdd(&sh.count, incl);
+        at = __builtin_amdgcn_readlane(at, 63) + incl - mine;
+        auto add = [&](float v, int j) {
+          if (v >= floor_x) {
+            if (at < CAP) {
+              u.listed.x[at] = v;
+              u.listed.id[at] = j;
+            }
+            ++at;
+          }
+        };
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = j0 + 4 * (tid + i * THREADS);
+          add(y[i].x, j);
+          add(y[i].y, j + 1);
+          add(y[i].z, j + 2);
+          add(y[i].w, j + 3);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = z[i];
       }
-      if (tid == 0) sh.found = 0;
-      const float share = (float)k * 4.0f / (float)vpt;
-      __syncthreads();
-      find_bin<THREADS>((int)(share + 6.0f * sqrtf(2.0f * share) + 8.0f), sh);
-      floor_bin = sh.found;
-      __syncthreads();
+      for (int i = tid; i < (n + 31) / 32; i += THREADS) map[i] = 0;
       for (int i = tid; i < BINS; i += THREADS) sh.bins[i] = 0;
       __syncthreads();
-    }
-    auto count = [&](int from) {
+      const int all = sh.count;
+      if (all > CAP || all < k) return false;
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
-        const int b = m.bin(x[i]);
-        if (x[i] != SEL_NONE && b >= from && (from == floor_bin || b < floor_bin)) atomicAdd(&sh.bins[b], 1u);
-      }
-      if (tid == 0) sh.found = -1;
-      __syncthreads();
-      find_bin<THREADS>(k, sh);
-    };
-    count(floor_bin);
-    if (floor_bin > 0 && sh.found < 0) {  // (the sample put it too high: the others are counted too)
-      __syncthreads();
-      count(0);
-    }
-    const int bin = sh.found, in_bin = sh.in_bin, need = k - sh.below;
-    if (in_bin > LIST) {
-      return false;
-    }
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      if (x[i] != SEL_NONE && m.bin(x[i]) == bin) sh.list_x[atomicAdd(&sh.count, 1)] = x[i];
-    }
-    __syncthreads();
-    for (int i = tid; i < in_bin; i += THREADS) {
-      const float y = sh.list_x[i];
-      int above = 0, same = 0;
-      for (int e = 0; e < in_bin; ++e) {
-        above += sh.list_x[e] > y;
-        same += sh.list_x[e] == y;
-      }
-      if (above < need && need <= above + same) sh.value = y;
-    }
-    __syncthreads();
-    const float kth = sh.value;
-
-    // 2. rows within the bound of it
-    const float b_lo = kth - 2.0f * err, b_hi = kth + 2.0f * err;
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
-    int sure = 0;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      sure += x[i] > b_hi;
-      if (x[i] >= b_lo && x[i] <= b_hi && x[i] != SEL_NONE) {
-        const int e = atomicAdd(&sh.count, 1);
-        if (e < LIST) sh.list_j[e] = id_of(i);
+        const int e = tid + i * THREADS;
+        x[i] = e < all ? u.listed.x[e] : SEL_NONE;
+        if (SAMPLED) id[i] = e < all ? u.listed.id[e] : 0;
       }
     }
-    sure = block_sum<THREADS>(sure, sh.wave_b);
-    __syncthreads();
-    const int close = sh.count, rest = k - sure;  // `rest` of the `close` rows are taken
-    if (close > LIST || (SAMPLED && listed && list_map.bin(b_lo) < list_bin)) {
-      return false;
-    }
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      if (x[i] > b_hi) take(id_of(i));
-    }
-    if (close == rest) {
-      for (int i = tid; i < close; i += THREADS) take(sh.list_j[i]);
-    } else {
-      const int groups = (close + 15) / 16, heads16 = (a.heads + 15) / 16;
-      if (WAVES == 1) {
-        for (int i = 0; i < close; i += 16) {
-          const uint64_t key = order64<T, FP8>(a, p, t, table, sh.list_j[min(i + (lane & 15), close - 1)], lane);
-          if (lane < 16 && i + lane < close) sh.list_key[i + lane] = key;
-        }
+    auto id_of = [&](int i) { return listed ? id[SAMPLED ? i : 0] : (i >> 2) * 4 * THREADS + 4 * tid + (i & 3); };
+    auto take = [&](int j) {
+      if (listed) {
+        atomicOr(&map[j >> 5], 1u << (j & 31));
       } else {
-        for (int i = wave; i < groups * heads16; i += WAVES) {
-          const int e = i / heads16 * 16, h16 = i % heads16;
-          const double s = score64_part<T, FP8>(a, p, t, table, sh.list_j[min(e + (lane & 15), close - 1)],
-                                                16 * h16, lane);
-          if (lane < 16 && e + lane < close) u.part[h16][e + lane] = s;
+        atomicOr(&map[(j >> 8) * 8 + (j & 3) * 2 + ((j >> 7) & 1)], 1u << ((j >> 2) & 31));
+      }
+    };
+    // the votes of a wave's four values i..i + 3
+    auto put_votes = [&](int i, uint64_t m0, uint64_t m1, uint64_t m2, uint64_t m3) {
+      const uint64_t m = lane == 0 ? m0 : lane == 1 ? m1 : lane == 2 ? m2 : m3;
+      if (lane < 4) ((uint64_t*)map)[((i >> 2) * WAVES + wave) * 4 + lane] = m;
+    };
+
+    // the range, and how many rows there are to choose from
+    float lo = SEL_MAX, hi = -SEL_MAX;
+    int there = 0;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const bool is = x[i] != SEL_NONE;
+      lo = fminf(lo, is ? x[i] : SEL_MAX);
+      hi = fmaxf(hi, x[i]);
+      there += is;
+    }
+    block_range<THREADS>(lo, hi, sh);  // (a barrier: the list's length has been read)
+    if (tid == 0) sh.count = 0;
+    there = block_sum<THREADS>(there, SLOT_THERE, sh);
+    if (there > 0 && (lo <= -SEL_MAX || hi >= SEL_MAX)) {  // a score left fp32's range
+      err = __builtin_inff();
+      return false;
+    }
+    if (there <= k) {
+#pragma unroll
+      for (int i = 0; i < VPT; i += 4) {
+        if (!listed && i / 4 < runs) {
+          put_votes(i, __ballot(x[i] != SEL_NONE), __ballot(x[i + 1] != SEL_NONE),
+                    __ballot(x[i + 2] != SEL_NONE), __ballot(x[i + 3] != SEL_NONE));
+        }
+      }
+      if (listed) return false;  // (it has topk values or more)
+    } else {
+      // 1. [e_lo, e_hi] around the topk-th largest, wide enough for the bound on both sides:
+      // bins over the range, and over one bin's range where that holds too many
+      int need = k, bin;
+      BinMap<THREADS> m;
+      for (int round = 0;; ++round) {
+        m = BinMap<THREADS>::of(lo, hi);
+        if (!(lo < hi) || !m.usable() || round == 4) return false;
+        // (of many values per thread only those above a bin that a sample of them puts a
+        // little below the topk-th are counted, by the rule of the list's sample)
+        int floor_bin = 0;
+        if (VPT >= 16 && THREADS == 1024 && runs >= 4 && round == 0) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (x[i] != SEL_NONE) atomicAdd(&sh.bins[m.bin(x[i])], 1u);
+          }
+          const float share = (float)k * (4.0f * THREADS) / (float)n;
+          __syncthreads();
+          find_bin<THREADS>((int)(share + 6.0f * sqrtf(2.0f * share) + 8.0f), SLOT_SAMPLE, sh);
+          floor_bin = sh.found;
+          for (int i = tid; i < BINS; i += THREADS) sh.bins[i] = 0;
+          __syncthreads();
+        }
+        auto count = [&](int from, int to) {
+#pragma unroll
+          for (int i = 0; i < VPT; ++i) {
+            const int b = m.bin(x[i]);
+            if (x[i] >= lo && x[i] <= hi && b >= from && b < to) atomicAdd(&sh.bins[b], 1u);
+          }
+          if (tid == 0) sh.found = -1;
+          __syncthreads();
+          find_bin<THREADS>(need, SLOT_COUNT, sh);
+        };
+        count(floor_bin, BINS);
+        if (sh.found < 0) {  // (the sample put it too high: the others are counted too)
+          __syncthreads();
+          count(0, floor_bin);
+        }
+        bin = sh.found;
+        need -= sh.below;
+        if (sh.in_bin <= LIST / 2) break;
+        float l2 = SEL_MAX, h2 = -SEL_MAX;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+          if (x[i] >= lo && x[i] <= hi && m.bin(x[i]) == bin) l2 = fminf(l2, x[i]), h2 = fmaxf(h2, x[i]);
+        }
+        block_range<THREADS>(l2, h2, sh);
+        lo = l2;
+        hi = h2;
+        for (int i = tid; i < BINS; i += THREADS) sh.bins[i] = 0;
+        __syncthreads();
+      }
+      const float slop = 2.0f * err + 4e-6f * (fabsf(lo) + fabsf(hi));
+      const float e_lo = m.edge(bin) - slop, e_hi = m.edge(bin + 1) + slop;
+      if (!(e_lo > -SEL_MAX) || !(e_hi < SEL_MAX) || (listed && e_lo < floor_x)) return false;
+
+      // 2. values above are taken, those inside are listed
+      int above = 0;
+      auto classify = [&](int i) -> uint64_t {
+        const bool over = x[i] > e_hi;
+        const uint64_t vote = __ballot(over);
+        above += (int)__popcll(vote);
+        if (listed && over) take(id_of(i));
+        if (!over && x[i] >= e_lo) {
+          const int e = atomicAdd(&sh.count, 1);
+          if (e < LIST) {
+            sh.list_x[e] = x[i];
+            sh.list_j[e] = id_of(i);
+          }
+        }
+        return vote;
+      };
+#pragma unroll
+      for (int i = 0; i < VPT; i += 4) {
+        if (!listed && i / 4 >= runs) continue;
+        const uint64_t v0 = classify(i), v1 = classify(i + 1), v2 = classify(i + 2), v3 = classify(i + 3);
+        if (!listed) put_votes(i, v0, v1, v2, v3);
+      }
+      above = block_sum<THREADS>(lane == 0 ? above : 0, SLOT_ABOVE, sh);
+      __syncthreads();
+      const int inside = sh.count;
+      need = k - above;
+      if (inside > LIST || need < 1 || need > inside) return false;
+      if (tid == 0) sh.close = sh.sure = 0;
+      rank_list<THREADS>(inside, sh.list_x, sh.list_j, [&](int i, int rank) {
+        if (rank == need - 1) sh.value = sh.list_x[i];
+      });
+      __syncthreads();
+      const float kth = sh.value, b_lo = kth - 2.0f * err, b_hi = kth + 2.0f * err;
+      if (b_lo < e_lo || b_hi > e_hi) return false;
+      for (int i = tid; i < inside; i += THREADS) {
+        const float y = sh.list_x[i];
+        if (y > b_hi) {
+          take(sh.list_j[i]);
+          atomicAdd(&sh.sure, 1);
+        } else if (y >= b_lo) {
+          sh.close_j[atomicAdd(&sh.close, 1)] = sh.list_j[i];
+        }
+      }
+      __syncthreads();
+      const int close = sh.close, rest = need - sh.sure;  // `rest` of the `close` rows are taken
+      if (close == rest) {
+        for (int i = tid; i < close; i += THREADS) take(sh.close_j[i]);
+      } else {
+        const int groups = (close + 15) / 16, heads16 = (a.heads + 15) / 16;
+        if (WAVES == 1) {
+          for (int i = 0; i < close; i += 16) {
+            const uint64_t key = order64<T, FP8>(a, p, t, table, sh.close_j[min(i + (lane & 15), close - 1)], lane);
+            if (lane < 16 && i + lane < close) sh.list_key[i + lane] = key;
+          }
+        } else {
+          for (int i = wave; i < groups * heads16; i += WAVES) {
+            const int e = i / heads16 * 16, h16 = i % heads16;
+            const double s = score64_part<T, FP8>(a, p, t, table, sh.close_j[min(e + (lane & 15), close - 1)],
+                                                  16 * h16, lane);
+            if (lane < 16 && e + lane < close) u.part[h16][e + lane] = s;
+          }
+          __syncthreads();
+          for (int i = tid; i < close; i += THREADS) {
+            double s = 0.0;
+            for (int h16 = 0; h16 < heads16; ++h16) s += u.part[h16][i];
+            sh.list_key[i] = order_of(s * key_scale64<FP8>(a, p, table, sh.close_j[i]));
+          }
         }
         __syncthreads();
-        for (int i = tid; i < close; i += THREADS) {
-          double s = 0.0;
-          for (int h16 = 0; h16 < heads16; ++h16) s += u.part[h16][i];
-          sh.list_key[i] = order_of(s * key_scale64<FP8>(a, p, table, sh.list_j[i]));
-        }
-      }
-      __syncthreads();
-      for (int i = tid; i < close; i += THREADS) {
-        const uint64_t key = sh.list_key[i];
-        const int j = sh.list_j[i];
-        int rank = 0;
-        for (int e = 0; e < close; ++e) {
-          const uint64_t o = sh.list_key[e];
-          rank += o > key || (o == key && sh.list_j[e] < j);
-        }
-        if (rank < rest) take(j);
+        rank_list<THREADS>(close, sh.list_key, sh.close_j, [&](int i, int rank) {
+          if (rank < rest) take(sh.close_j[i]);
+        });
       }
     }
-  }
-  __syncthreads();
+    __syncthreads();
 
-  // 3. the ids in order
-  const int per = (map_words + THREADS - 1) / THREADS, w0 = min(tid * per, map_words),
-            w1 = min(w0 + per, map_words);
-  int mine = 0, all;
-  for (int w = w0; w < w1; ++w) mine += __popc(map[w]);
-  int pos = block_before<THREADS>(mine, sh.wave_a, all);
-  for (int w = w0; w < w1; ++w) {
-    for (uint32_t bits = map[w]; bits; bits &= bits - 1) ids[pos++] = 32 * w + __builtin_ctz(bits);
-  }
-  for (int i = all + tid; i < k; i += THREADS) ids[i] = -1;
-  return true;
+    // 3. the ids in order
+    const int words = listed ? (n + 31) / 32 : (n + 255) / 256 * 8;
+    const int per = (words + THREADS - 1) / THREADS, w0 = min(tid * per, words), w1 = min(w0 + per, words);
+    auto word = [&](int w) -> uint32_t {
+      if (listed) return map[w];
+      const unsigned char* votes = (const unsigned char*)map + (w >> 3) * 32 + (w & 7);
+      return every_fourth(votes[0]) | every_fourth(votes[8]) << 1 | every_fourth(votes[16]) << 2 |
+             every_fourth(votes[24]) << 3;
+    };
+    int mine = 0, all;
+    for (int w = w0; w < w1; ++w) mine += __popc(word(w));
+    int pos = block_before<THREADS>(mine, SLOT_IDS, sh, all);
+    for (int w = w0; w < w1; ++w) {
+      for (uint32_t bits = word(w); bits; bits &= bits - 1) ids[pos++] = 32 * w + __builtin_ctz(bits);
+    }
+    for (int i = all + tid; i < k; i += THREADS) ids[i] = -1;
+    return true;
   };
-  if (!from_registers()) select_from_memory<T, FP8, THREADS>(a, p, t, n, err, g, table, sh);
+  if (!from_registers()) {
+    __syncthreads();
+    select_from_memory<T, FP8, THREADS>(a, p, t, n, err, g, table, sh);
+  }
 }
 
 // ---------------------------------------------------------------------------
