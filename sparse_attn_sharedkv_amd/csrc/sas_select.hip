@@ -66,6 +66,11 @@ struct Elem<__bf16> {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, a),
                                            __builtin_bit_cast(bf16x2, a), c, false);
   }
+  // two e4m3 codes (the low or the high half of w), scaled by 1
+  static __device__ uint32_t widen(uint32_t w, bool high) {
+    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+  }
   static __device__ float lo(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
   static __device__ float hi(uint32_t w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
 };
@@ -80,6 +85,10 @@ struct Elem<_Float16> {
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, a), __builtin_bit_cast(f16x2, a), c,
                                   false);
   }
+  static __device__ uint32_t widen(uint32_t w, bool high) {
+    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+  }
   static __device__ float lo(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[0]; }
   static __device__ float hi(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[1]; }
 };
@@ -87,14 +96,13 @@ struct Elem<_Float16> {
 // Eight e4m3 codes as eight elements of T (exact: e4m3 fits in both 16-bit types).
 template <typename T>
 __device__ inline u32x4 widen_e4m3(u32x2 c) {
-  typename Elem<T>::v8 r;
+  u32x4 r;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(c[i], false);
-    const auto b = __builtin_amdgcn_cvt_pk_f32_fp8(c[i], true);
-    r[4 * i] = (T)a[0], r[4 * i + 1] = (T)a[1], r[4 * i + 2] = (T)b[0], r[4 * i + 3] = (T)b[1];
+    r[2 * i] = Elem<T>::widen(c[i], false);
+    r[2 * i + 1] = Elem<T>::widen(c[i], true);
   }
-  return __builtin_bit_cast(u32x4, r);
+  return r;
 }
 
 // The bound on an fp32 score's error: 0 where every score is exactly 0, infinite where it says
@@ -111,11 +119,12 @@ struct SelPlan {
   int t_begin, t_end;   // query rows of this pass
   int width;            // scores kept for a row (row stride of the workspace)
   int chunks;           // workgroups that share a row's keys
-  int slices;           // waves that share a chunk's keys (each leaves its own key norm)
+  int slices;           // waves that share a piece's keys
+  int norms;            // key norms that a piece leaves (one of each wave that has looked at keys)
   int wq;               // query rows of a workgroup
   FastDiv page_div, ratio_div;
   float* w_norm;        // [rows of the pass] W of each row
-  float* k_norm;        // [batch][chunks][slices] largest |k|^2 of the keys seen
+  float* k_norm;        // [batch][chunks][norms] largest |k|^2 of the keys seen
   float* score;         // [rows of the pass][width]
 };
 
@@ -189,6 +198,12 @@ __device__ inline int piece_keys(const SelPlan& p, int thr) {
 // The K dimension is taken in an order that gives a lane whole runs of a key row: step 2 p + u,
 // half hf of the wave holds dims [32 p + 16 hf + 8 u, +8) of both operands.
 
+// max(0, x), in one instruction (a float's bits order like a signed integer's at zero; fmaxf
+// takes two, the first to quiet what NaN there may be; positive NaN stays NaN here)
+__device__ inline float above_zero(float x) {
+  return __builtin_bit_cast(float, max(__builtin_bit_cast(int, x), 0));
+}
+
 __device__ inline int frag_dim(int p, int u, int hf) { return 32 * p + 16 * hf + 8 * u; }
 
 template <typename T, int D, int MT>
@@ -202,16 +217,16 @@ struct QueryFrags {
     const float* wb = a.weights + (int64_t)t * a.heads;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      const int h = 32 * mt + m;
+      // (heads there are not: the last one's, with weight 0)
+      const int h = min(32 * mt + m, a.heads - 1);
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        q[mt][k] = h < a.heads ? *(const u32x4*)(base + (int64_t)h * D + frag_dim(k >> 1, k & 1, hf))
-                               : u32x4{0, 0, 0, 0};
-      }
+      for (int k = 0; k < D / 16; ++k)
+        q[mt][k] = *(const u32x4*)(base + (int64_t)h * D + frag_dim(k >> 1, k & 1, hf));
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int hh = 32 * mt + 8 * (i >> 2) + 4 * hf + (i & 3);
-        w[mt][i] = hh < a.heads ? wb[hh] : 0.0f;
+        const float v = wb[min(hh, a.heads - 1)];
+        w[mt][i] = hh < a.heads ? v : 0.0f;
       }
     }
   }
@@ -247,7 +262,7 @@ struct QueryFrags {
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) acc = Elem<T>::mfma(q[mt][kk], k[kk], acc);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i & 3] = fmaf(fmaxf(acc[i], 0.0f), w[mt][i], s[i & 3]);
+      for (int i = 0; i < 16; ++i) s[i & 3] = fmaf(above_zero(acc[i]), w[mt][i], s[i & 3]);
     }
     const float r = (s[0] + s[1]) + (s[2] + s[3]);
     return r + __shfl_xor(r, 32, 64);
@@ -256,12 +271,13 @@ struct QueryFrags {
 
 template <typename T, int D>
 __device__ inline float key_norm2(const u32x4 k[D / 16]) {
-  float n = 0.0f;
+  float n[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) n = Elem<T>::dot2(k[kk][e], n);
-  return n + __shfl_xor(n, 32, 64);
+    for (int e = 0; e < 4; ++e) n[e] = Elem<T>::dot2(k[kk][e], n[e]);
+  const float s = (n[0] + n[1]) + (n[2] + n[3]);
+  return s + __shfl_xor(s, 32, 64);
 }
 
 __device__ inline float kept_score(float s) {
@@ -275,12 +291,23 @@ __device__ inline float max_nonneg(float a, float b) {
                                        __builtin_bit_cast(uint32_t, b) & 0x7fffffffu));
 }
 
+// Byte offset in LDS of 16-byte chunk c of row r, C chunks to a row: the rows' chunks are rotated
+// against each other, so that 16 lanes reading one chunk of 16 rows touch every bank once.
+template <int C>
+__device__ inline int chunk_at(int r, int c) {
+  return r * (16 * C) + ((c ^ (r / (16 / C) & (C - 1))) << 4);
+}
+
 // Decode: few query rows a sequence. A workgroup's four waves take wq query rows times 4 / wq
 // slices of a chunk's keys; nothing is shared and there is no barrier. Keys go from memory to
 // registers, the next tile's in flight under the current one's products. Bound by the keys'
 // bytes: a key row is read once for each query row.
+template <bool FP8>
+constexpr int STREAM_DEPTH = FP8 ? 2 : 1;  // tiles of 32 keys that a wave has on their way
+
 template <typename T, bool FP8, int D, int MT>
-__global__ __launch_bounds__(256) void score_stream_kernel(SasSelectArgs a, SelPlan p) {
+__global__ __launch_bounds__(256, MT <= 2 ? 2 : 1) void score_stream_kernel(SasSelectArgs a, SelPlan p) {
+  __shared__ __attribute__((aligned(256))) unsigned char stage[4][32 * (FP8 ? D : 2 * D)];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 31, hf = lane >> 5;
   const int piece = (int)(blockIdx.x % (unsigned)p.chunks);
   const int t = p.t_begin + (int)(blockIdx.x / (unsigned)p.chunks) * p.wq + wave % p.wq;
@@ -301,62 +328,94 @@ __global__ __launch_bounds__(256) void score_stream_kernel(SasSelectArgs a, SelP
   const int32_t* table = a.block_table + (int64_t)r.b * a.table_len;
   float* out = p.score + (int64_t)(t - p.t_begin) * p.width;
 
+  // DEPTH tiles on their way from memory, and the pages of the DEPTH behind them
+  constexpr int ROW = FP8 ? D : 2 * D, LOADS = ROW / 32, DEPTH = STREAM_DEPTH<FP8>;
+  constexpr int C = ROW / 16, R = 64 / C;  // 16-byte chunks of a row, rows of a load
+  const uint32_t page_units = (uint32_t)(a.block_size * (FP8 ? D + 4 : 2 * D) / 16);
+  const unsigned char* lane_keys = (const unsigned char*)a.keys + 16 * (lane % C);
+  unsigned char* own = stage[wave];
+  u32x4 raw[DEPTH][LOADS];
+  float scale[DEPTH];
+  bool ok[DEPTH];
+  int page[DEPTH];
   auto page_of = [&](int j) { return j < hi ? table[p.page_div.div(j)] : -1; };
-  auto load = [&](int j, int page, u32x4 k[D / 16], float& scale) {
-    const bool ok = page >= 0 && page < a.block_num;
-    const int at = j - p.page_div.div(j) * a.block_size;
-    if (!FP8) {
-      const T* row = (const T*)a.keys + (ok ? (int64_t)page * a.block_size + at : 0) * D;
+  auto load = [&](int u, int j) {
+    ok[u] = page[u] >= 0 && page[u] < a.block_num;
+    const uint32_t at = ok[u] ? j - p.page_div.div(j) * a.block_size : 0;
+    const uint32_t pg = (ok[u] ? (uint32_t)page[u] : 0) * page_units;
+    // where the lane's key starts, in 16 bytes (the pool has fewer than 2^32 of them)
+    const int unit = (int)(pg + at * C);
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) k[kk] = *(const u32x4*)(row + frag_dim(kk >> 1, kk & 1, hf));
-    } else {
-      const unsigned char* pg = (const unsigned char*)a.keys +
-                                (ok ? (int64_t)page : 0) * a.block_size * (D + 4);
-      const unsigned char* row = pg + (ok ? at : 0) * D;
-#pragma unroll
-      for (int q = 0; q < D / 32; ++q) k[q] = *(const u32x4*)(row + 32 * q + 16 * hf);
-      scale = *(const float*)(pg + (int64_t)a.block_size * D + 4 * (ok ? at : 0));
+    for (int q = 0; q < LOADS; ++q) {
+      const uint32_t from = (uint32_t)__shfl(unit, R * q + lane / C, 64);
+      raw[u][q] = *(const u32x4*)(lane_keys + (uint64_t)from * 16);
     }
-    return ok;
+    if (FP8) {
+      scale[u] = *(const float*)((const unsigned char*)a.keys + (uint64_t)(pg + a.block_size * C) * 16 +
+                                 4 * at);
+    }
+  };
+  // whole rows into LDS as they came, a lane's parts of its key out of it (a wave's own piece of
+  // LDS: its accesses keep their order)
+  auto turn = [&](int u, u32x4 part[LOADS]) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int q = 0; q < LOADS; ++q)
+      *(u32x4*)(own + chunk_at<C>(R * q + lane / C, lane % C)) = raw[u][q];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      // fp8: 16 codes, the steps 2 i and 2 i + 1
+      const int c = FP8 ? 2 * i + hf : frag_dim(i >> 1, i & 1, hf) / 8;
+      part[i] = *(const u32x4*)(own + chunk_at<C>(n, c));
+    }
   };
 
-  int j = lo + 32 * slice + n;
-  int page_next = page_of(j + step);
-  u32x4 cur[D / 16], nxt[D / 16];
-  float sc_cur = 1.0f, sc_nxt = 1.0f;
-  bool ok_cur = load(j, page_of(j), cur, sc_cur), ok_nxt = false;
-  for (int base = lo + 32 * slice; base < hi; base += step, j += step) {
-    const int page_far = page_of(j + 2 * step);
-    ok_nxt = load(j + step, page_next, nxt, sc_nxt);
-    page_next = page_far;
-    u32x4 k[D / 16];
-    if (FP8) {
+  const int first = lo + 32 * slice;
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        const u32x4 c = cur[kk >> 1];
-        k[kk] = widen_e4m3<T>(kk & 1 ? u32x2{c[2], c[3]} : u32x2{c[0], c[1]});
+  for (int u = 0; u < DEPTH; ++u) page[u] = page_of(first + u * step + n);
+#pragma unroll
+  for (int u = 0; u < DEPTH; ++u) {
+    load(u, first + u * step + n);
+    page[u] = page_of(first + (DEPTH + u) * step + n);
+  }
+  u32x4 part[LOADS];
+  if (FP8 && first < hi) turn(0, part);
+  for (int base = first; base < hi; base += DEPTH * step) {
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u) {
+      const int j = base + u * step + n;
+      if (base + u * step >= hi) break;
+      const float sc = FP8 ? scale[u] : 1.0f;
+      const bool is = ok[u];
+      if (!FP8) turn(u, part);
+      load(u, j + DEPTH * step);
+      page[u] = page_of(j + 2 * DEPTH * step);
+      u32x4 k[D / 16];
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        if (FP8) {
+          k[2 * i] = widen_e4m3<T>(u32x2{part[i][0], part[i][1]});
+          k[2 * i + 1] = widen_e4m3<T>(u32x2{part[i][2], part[i][3]});
+        } else {
+          k[i] = part[i];
+        }
       }
-    } else {
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) k[kk] = cur[kk];
+      if (FP8) turn((u + 1) % DEPTH, part);  // the next tile's, under this one's products
+      if (norms) {
+        float n2 = key_norm2<T, D>(k);
+        if (FP8) n2 *= sc * sc;
+        if (is) kn = max_nonneg(kn, n2);
+      }
+      float s = qf.score(k);
+      if (FP8) s *= sc;
+      if (hf == 0 && j < hi) out[j] = is ? kept_score(s) : SEL_NONE;
     }
-    if (norms) {
-      float n2 = key_norm2<T, D>(k);
-      if (FP8) n2 *= sc_cur * sc_cur;
-      if (ok_cur) kn = max_nonneg(kn, n2);
-    }
-    float s = qf.score(k);
-    if (FP8) s *= sc_cur;
-    if (hf == 0 && j < hi) out[j] = ok_cur ? kept_score(s) : SEL_NONE;
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) cur[kk] = nxt[kk];
-    sc_cur = sc_nxt;
-    ok_cur = ok_nxt;
   }
   if (norms) {
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) kn = max_nonneg(kn, __shfl_xor(kn, off, 64));
-    if (lane == 0) p.k_norm[((int64_t)r.b * p.chunks + piece) * p.slices + slice] = kn;
+    if (lane == 0) p.k_norm[((int64_t)r.b * p.chunks + piece) * p.norms + slice] = kn;
   }
 }
 
@@ -366,13 +425,6 @@ __global__ __launch_bounds__(256) void score_stream_kernel(SasSelectArgs a, SelP
 // A tile of eight rows that spans sequences takes them one after the other.
 constexpr int TILE_WAVES = 8;
 constexpr int TILE_KEYS = 64;
-
-// byte offset of 16-byte chunk c of row r in a stage: the rows' chunks are rotated against each
-// other so that 16 lanes reading one chunk of 16 rows touch every bank once
-template <int D>
-__device__ inline int stage_at(int r, int c) {
-  return D == 128 ? r * 256 + ((c ^ (r & 15)) << 4) : r * 128 + ((c ^ ((r >> 1) & 7)) << 4);
-}
 
 template <typename T, bool FP8, int D, int MT>
 __global__ __launch_bounds__(64 * TILE_WAVES) void score_tile_kernel(SasSelectArgs a, SelPlan p) {
@@ -404,7 +456,7 @@ __global__ __launch_bounds__(64 * TILE_WAVES) void score_tile_kernel(SasSelectAr
     const bool mine = t >= ts && t < te;
     const int my_thr = mine ? thr_at(a, p, t) : 0;
     const bool active = mine && my_thr > a.topk && lo < my_thr;
-    const bool norms = mine && t == min(seg.last, p.t_end) - 1;
+    const bool norms = te == min(seg.last, p.t_end);  // the tile that sees all of the sequence's keys
     if (active) {
       qf.load(a, t, lane);
       if (piece == 0) {
@@ -435,14 +487,33 @@ __global__ __launch_bounds__(64 * TILE_WAVES) void score_tile_kernel(SasSelectAr
       }
     };
     auto put = [&](int buf) {
+      if (norms) {
+        u32x4 k[2] = {};
+        if (!FP8) {
+#pragma unroll
+          for (int i = 0; i < LOADS; ++i) k[i] = held[i];
+        } else if (loads_codes) {
+          k[0] = widen_e4m3<T>(u32x2{held[0][0], held[0][1]});
+          k[1] = widen_e4m3<T>(u32x2{held[0][2], held[0][3]});
+        }
+        float n2 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) n2 = Elem<T>::dot2(k[i][e], n2);
+#pragma unroll
+        for (int off = 1; off < PARTS; off <<= 1) n2 += __shfl_xor(n2, off, 64);
+        if (FP8) n2 *= held_scale * held_scale;
+        if (held_ok) kn = max_nonneg(kn, n2);
+      }
       if (!FP8) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
-          *(u32x4*)(stage[buf] + stage_at<D>(row, part * LOADS + i)) = held[i];
+          *(u32x4*)(stage[buf] + chunk_at<D / 8>(row, part * LOADS + i)) = held[i];
       } else if (loads_codes) {
-        *(u32x4*)(stage[buf] + stage_at<D>(row, 2 * part)) =
+        *(u32x4*)(stage[buf] + chunk_at<D / 8>(row, 2 * part)) =
             widen_e4m3<T>(u32x2{held[0][0], held[0][1]});
-        *(u32x4*)(stage[buf] + stage_at<D>(row, 2 * part + 1)) =
+        *(u32x4*)(stage[buf] + chunk_at<D / 8>(row, 2 * part + 1)) =
             widen_e4m3<T>(u32x2{held[0][2], held[0][3]});
       }
       if (part == 0) {
@@ -463,33 +534,29 @@ __global__ __launch_bounds__(64 * TILE_WAVES) void score_tile_kernel(SasSelectAr
         page_next = page_of(base + 2 * TILE_KEYS + row);
       }
       if (active) {
+        // both halves of the stage without a branch between them, so that one's weighted sums can
+        // run under the other's products; then each half of the wave keeps 32 scores
+        float half_score[2];
 #pragma unroll
         for (int kt = 0; kt < TILE_KEYS / 32; ++kt) {
-          if (base + 32 * kt >= my_thr) break;
-          const int kr = 32 * kt + n, j = base + kr;
           u32x4 k[D / 16];
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
-            k[kk] = *(const u32x4*)(stage[buf] + stage_at<D>(kr, frag_dim(kk >> 1, kk & 1, hf) / 8));
-          const bool ok = key_ok[buf][kr];
-          const float sc = FP8 ? key_scale[buf][kr] : 1.0f;
-          if (norms) {
-            float n2 = key_norm2<T, D>(k);
-            if (FP8) n2 *= sc * sc;
-            if (ok) kn = max_nonneg(kn, n2);
-          }
-          float s = qf.score(k);
-          if (FP8) s *= sc;
-          if (hf == 0 && j < my_thr && j < hi) out[j] = ok ? kept_score(s) : SEL_NONE;
+            k[kk] = *(const u32x4*)(stage[buf] + chunk_at<D / 8>(32 * kt + n, frag_dim(kk >> 1, kk & 1, hf) / 8));
+          half_score[kt] = qf.score(k);
         }
+        float s = hf ? half_score[1] : half_score[0];
+        if (FP8) s *= key_scale[buf][lane];
+        const int j = base + lane;
+        if (j < my_thr && j < hi) out[j] = key_ok[buf][lane] ? kept_score(s) : SEL_NONE;
       }
       if (more) put(buf ^ 1);
       __syncthreads();
     }
     if (norms) {
 #pragma unroll
-      for (int off = 1; off < 32; off <<= 1) kn = max_nonneg(kn, __shfl_xor(kn, off, 64));
-      if (lane == 0) p.k_norm[(int64_t)seg.b * p.chunks + piece] = kn;
+      for (int off = 1; off < 64; off <<= 1) kn = max_nonneg(kn, __shfl_xor(kn, off, 64));
+      if (lane == 0) p.k_norm[((int64_t)seg.b * p.chunks + piece) * p.norms + wave] = kn;
     }
     ts = te;
   }
@@ -1057,8 +1124,8 @@ __global__ __launch_bounds__(THREADS, THREADS == 64 ? 5 : 4) void select_kernel(
     float kn = 0.0f;
     {
       const int thr_end = thr_at(a, p, min(r.last, p.t_end) - 1), keys = piece_keys(p, thr_end);
-      const int parts = (thr_end + keys - 1) / keys * p.slices;
-      const float* kp = p.k_norm + (int64_t)r.b * p.chunks * p.slices;
+      const int parts = (thr_end + keys - 1) / keys * p.norms;
+      const float* kp = p.k_norm + (int64_t)r.b * p.chunks * p.norms;
       for (int i = lane; i < parts; i += 64) kn = max_nonneg(kn, kp[i]);
       kn = as_float(__builtin_amdgcn_readlane(
           wave_scan(as_int(kn), 0, [](int a, int b) { return max(a, b); }), 63));
@@ -1364,14 +1431,15 @@ PassPlan plan_passes(const SasSelectArgs& a) {
   r.tiles = per_seq >= 4;
   p.wq = r.tiles ? TILE_WAVES : per_seq >= 2 ? 2 : 1;
   p.slices = r.tiles ? 1 : 4 / p.wq;
+  p.norms = r.tiles ? TILE_WAVES : p.slices;
   const int64_t groups = (r.rows + p.wq - 1) / p.wq;
   // enough workgroups to fill the chip a few times over, of at least 64 keys a slice
   const int64_t most = (p.width + 64 * p.slices - 1) / (64 * p.slices);
-  const int64_t pieces = ((r.tiles ? 512 : 1024) + groups - 1) / (groups < 1 ? 1 : groups);
+  const int64_t pieces = ((r.tiles ? 512 : 2048) + groups - 1) / (groups < 1 ? 1 : groups);
   p.chunks = (int)(pieces < 1 ? 1 : pieces > most ? most : pieces);
   // every part starts on 16 bytes
   const int64_t w_floats = ((int64_t)r.rows + 3) / 4 * 4;
-  const int64_t k_floats = ((int64_t)a.batch * p.chunks * p.slices + 3) / 4 * 4;
+  const int64_t k_floats = ((int64_t)a.batch * p.chunks * p.norms + 3) / 4 * 4;
   r.bytes = 4 * (w_floats + k_floats + (int64_t)r.rows * p.width);
   p.w_norm = (float*)a.workspace;
   p.k_norm = p.w_norm + w_floats;
@@ -1401,6 +1469,10 @@ int check_select(const SasSelectArgs* a) {
   if (a->max_keys < 1 || a->max_keys > (int64_t)a->table_len * a->block_size ||
       a->max_keys > SAS_SELECT_MAX_KEYS) {
     return fail("max_keys must be at least 1, and within the block table and SAS_SELECT_MAX_KEYS");
+  }
+  if ((int64_t)a->block_num * a->block_size * (a->key_format == SAS_ROW_FP8_INDEX ? a->dim + 4 : 2 * a->dim) >=
+      (1ll << 36)) {
+    return fail("an index cache of 64 GiB or more", SAS_E_UNSUPPORTED);
   }
   if (a->key_format == SAS_ROW_FP8_INDEX && (int64_t)a->block_size * (a->dim + 4) % 16) {
     return fail("fp8 index pages must be a multiple of 16 bytes");
