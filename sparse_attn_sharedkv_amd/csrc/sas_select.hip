@@ -206,10 +206,12 @@ __device__ inline float above_zero(float x) {
 
 __device__ inline int frag_dim(int p, int u, int hf) { return 32 * p + 16 * hf + 8 * u; }
 
-template <typename T, int D, int MT>
+// The weights are in registers too (W_LDS = 0), or in a wave's own piece of LDS.
+template <typename T, int D, int MT, bool W_LDS>
 struct QueryFrags {
   u32x4 q[MT][D / 16];
-  f32x16 w[MT];
+  f32x16 w[W_LDS ? 1 : MT];
+  float* w_lds;  // [32 MT]
 
   __device__ void load(const SasSelectArgs& a, int t, int lane) {
     const int m = lane & 31, hf = lane >> 5;
@@ -222,11 +224,16 @@ struct QueryFrags {
 #pragma unroll
       for (int k = 0; k < D / 16; ++k)
         q[mt][k] = *(const u32x4*)(base + (int64_t)h * D + frag_dim(k >> 1, k & 1, hf));
+      if (W_LDS) {
+        const float v = wb[h];
+        if (hf == 0) w_lds[32 * mt + m] = 32 * mt + m < a.heads ? v : 0.0f;
+      } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int hh = 32 * mt + 8 * (i >> 2) + 4 * hf + (i & 3);
-        const float v = wb[min(hh, a.heads - 1)];
-        w[mt][i] = hh < a.heads ? v : 0.0f;
+        for (int i = 0; i < 16; ++i) {
+          const int hh = 32 * mt + 8 * (i >> 2) + 4 * hf + (i & 3);
+          const float v = wb[min(hh, a.heads - 1)];
+          w[W_LDS ? 0 : mt][i] = hh < a.heads ? v : 0.0f;
+        }
       }
     }
   }
@@ -254,7 +261,7 @@ struct QueryFrags {
   }
 
   // the score of key lane & 31 without its scale
-  __device__ float score(const u32x4 k[D / 16]) const {
+  __device__ float score(const u32x4 k[D / 16], int hf) const {
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -262,7 +269,18 @@ struct QueryFrags {
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) acc = Elem<T>::mfma(q[mt][kk], k[kk], acc);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i & 3] = fmaf(above_zero(acc[i]), w[mt][i], s[i & 3]);
+      for (int g = 0; g < 4; ++g) {
+        float wv[4];
+        if (W_LDS) {
+          const float4 v = *(const float4*)(w_lds + 32 * mt + 8 * g + 4 * hf);
+          wv[0] = v.x, wv[1] = v.y, wv[2] = v.z, wv[3] = v.w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) wv[i] = w[W_LDS ? 0 : mt][4 * g + i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = fmaf(above_zero(acc[4 * g + i]), wv[i], s[i]);
+      }
     }
     const float r = (s[0] + s[1]) + (s[2] + s[3]);
     return r + __shfl_xor(r, 32, 64);
@@ -317,7 +335,7 @@ __global__ __launch_bounds__(256, MT <= 2 ? 2 : 1) void score_stream_kernel(SasS
   if (r.b < 0 || r.thr <= a.topk || lo >= r.thr) return;
   const int hi = min(lo + keys, r.thr), slice = wave / p.wq, step = 32 * p.slices;
 
-  QueryFrags<T, D, MT> qf;
+  QueryFrags<T, D, MT, false> qf;
   qf.load(a, t, lane);
   if (piece == 0 && slice == 0) {
     const float w = qf.bound(a, t, lane);
@@ -407,7 +425,7 @@ __global__ __launch_bounds__(256, MT <= 2 ? 2 : 1) void score_stream_kernel(SasS
         if (FP8) n2 *= sc * sc;
         if (is) kn = max_nonneg(kn, n2);
       }
-      float s = qf.score(k);
+      float s = qf.score(k, hf);
       if (FP8) s *= sc;
       if (hf == 0 && j < hi) out[j] = is ? kept_score(s) : SEL_NONE;
     }
@@ -431,6 +449,7 @@ __global__ __launch_bounds__(64 * TILE_WAVES) void score_tile_kernel(SasSelectAr
   __shared__ __attribute__((aligned(256))) unsigned char stage[2][TILE_KEYS * D * 2];
   __shared__ float key_scale[2][TILE_KEYS];
   __shared__ int key_ok[2][TILE_KEYS];
+  __shared__ __attribute__((aligned(16))) float weight[TILE_WAVES][32 * MT];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 31, hf = lane >> 5;
   const int piece = (int)(blockIdx.x % (unsigned)p.chunks);
   const int tiles = (p.t_end - p.t_begin + TILE_WAVES - 1) / TILE_WAVES;
@@ -443,7 +462,8 @@ __global__ __launch_bounds__(64 * TILE_WAVES) void score_tile_kernel(SasSelectAr
   const int row = threadIdx.x / PARTS, part = threadIdx.x % PARTS;
   const bool loads_codes = !FP8 || part < D / 16;
 
-  QueryFrags<T, D, MT> qf;
+  QueryFrags<T, D, MT, true> qf;
+  qf.w_lds = weight[wave];
   for (int ts = t0; ts < t1;) {
     const RowPos seg = locate(a, p, ts);
     const int te = max(min(seg.last, t1), ts + 1);
@@ -468,22 +488,23 @@ __global__ __launch_bounds__(64 * TILE_WAVES) void score_tile_kernel(SasSelectAr
     float* out = p.score + (int64_t)(t - p.t_begin) * p.width;
     float kn = 0.0f;
 
-    u32x4 held[LOADS];
-    float held_scale = 1.0f;
-    int held_ok = 0;
+    // two stages on their way: in registers until the one before them has been read
+    u32x4 held[2][LOADS];
+    float held_scale[2] = {1.0f, 1.0f};
+    int held_ok[2], page[2];
     auto page_of = [&](int j) { return j < hi ? table[p.page_div.div(j)] : -1; };
-    auto fetch = [&](int j, int page) {
-      held_ok = page >= 0 && page < a.block_num;
-      const int at = held_ok ? j - p.page_div.div(j) * a.block_size : 0;
-      const int64_t pg = held_ok ? page : 0;
+    auto fetch = [&](int u, int j) {
+      held_ok[u] = page[u] >= 0 && page[u] < a.block_num;
+      const int at = held_ok[u] ? j - p.page_div.div(j) * a.block_size : 0;
+      const int64_t pg = held_ok[u] ? page[u] : 0;
       if (!FP8) {
         const unsigned char* src = (const unsigned char*)a.keys + (pg * a.block_size + at) * (2 * D);
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) held[i] = *(const u32x4*)(src + 16 * (part * LOADS + i));
+        for (int i = 0; i < LOADS; ++i) held[u][i] = *(const u32x4*)(src + 16 * (part * LOADS + i));
       } else {
         const unsigned char* src = (const unsigned char*)a.keys + pg * a.block_size * (D + 4);
-        if (loads_codes) held[0] = *(const u32x4*)(src + at * D + 16 * part);
-        held_scale = *(const float*)(src + (int64_t)a.block_size * D + 4 * at);
+        if (loads_codes) held[u][0] = *(const u32x4*)(src + at * D + 16 * part);
+        held_scale[u] = *(const float*)(src + (int64_t)a.block_size * D + 4 * at);
       }
     };
     auto put = [&](int buf) {
@@ -491,10 +512,10 @@ __global__ __launch_bounds__(64 * TILE_WAVES) void score_tile_kernel(SasSelectAr
         u32x4 k[2] = {};
         if (!FP8) {
 #pragma unroll
-          for (int i = 0; i < LOADS; ++i) k[i] = held[i];
+          for (int i = 0; i < LOADS; ++i) k[i] = held[buf][i];
         } else if (loads_codes) {
-          k[0] = widen_e4m3<T>(u32x2{held[0][0], held[0][1]});
-          k[1] = widen_e4m3<T>(u32x2{held[0][2], held[0][3]});
+          k[0] = widen_e4m3<T>(u32x2{held[buf][0][0], held[buf][0][1]});
+          k[1] = widen_e4m3<T>(u32x2{held[buf][0][2], held[buf][0][3]});
         }
         float n2 = 0.0f;
 #pragma unroll
@@ -503,55 +524,61 @@ __global__ __launch_bounds__(64 * TILE_WAVES) void score_tile_kernel(SasSelectAr
           for (int e = 0; e < 4; ++e) n2 = Elem<T>::dot2(k[i][e], n2);
 #pragma unroll
         for (int off = 1; off < PARTS; off <<= 1) n2 += __shfl_xor(n2, off, 64);
-        if (FP8) n2 *= held_scale * held_scale;
-        if (held_ok) kn = max_nonneg(kn, n2);
+        if (FP8) n2 *= held_scale[buf] * held_scale[buf];
+        if (held_ok[buf]) kn = max_nonneg(kn, n2);
       }
       if (!FP8) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
-          *(u32x4*)(stage[buf] + chunk_at<D / 8>(row, part * LOADS + i)) = held[i];
+          *(u32x4*)(stage[buf] + chunk_at<D / 8>(row, part * LOADS + i)) = held[buf][i];
       } else if (loads_codes) {
         *(u32x4*)(stage[buf] + chunk_at<D / 8>(row, 2 * part)) =
-            widen_e4m3<T>(u32x2{held[0][0], held[0][1]});
+            widen_e4m3<T>(u32x2{held[buf][0][0], held[buf][0][1]});
         *(u32x4*)(stage[buf] + chunk_at<D / 8>(row, 2 * part + 1)) =
-            widen_e4m3<T>(u32x2{held[0][2], held[0][3]});
+            widen_e4m3<T>(u32x2{held[buf][0][2], held[buf][0][3]});
       }
       if (part == 0) {
-        key_ok[buf][row] = held_ok;
-        key_scale[buf][row] = held_scale;
+        key_ok[buf][row] = held_ok[buf];
+        key_scale[buf][row] = held_scale[buf];
       }
     };
 
-    int page_next = page_of(lo + TILE_KEYS + row);
-    fetch(lo + row, page_of(lo + row));
+#pragma unroll
+    for (int u = 0; u < 2; ++u) page[u] = page_of(lo + TILE_KEYS * u + row);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      fetch(u, lo + TILE_KEYS * u + row);
+      page[u] = page_of(lo + TILE_KEYS * (2 + u) + row);
+    }
     put(0);
     __syncthreads();
-    int buf = 0;
-    for (int base = lo; base < hi; base += TILE_KEYS, buf ^= 1) {
-      const bool more = base + TILE_KEYS < hi;
-      if (more) {
-        fetch(base + TILE_KEYS + row, page_next);
-        page_next = page_of(base + 2 * TILE_KEYS + row);
-      }
-      if (active) {
-        // both halves of the stage without a branch between them, so that one's weighted sums can
-        // run under the other's products; then each half of the wave keeps 32 scores
-        float half_score[2];
+    for (int base2 = lo; base2 < hi; base2 += 2 * TILE_KEYS) {
 #pragma unroll
-        for (int kt = 0; kt < TILE_KEYS / 32; ++kt) {
-          u32x4 k[D / 16];
+      for (int buf = 0; buf < 2; ++buf) {
+        const int base = base2 + TILE_KEYS * buf;
+        if (base >= hi) break;
+        fetch(buf, base + 2 * TILE_KEYS + row);
+        page[buf] = page_of(base + 4 * TILE_KEYS + row);
+        if (active) {
+          // both halves of the stage without a branch between them, so that one's weighted sums
+          // can run under the other's products; then each half of the wave keeps 32 scores
+          float half_score[2];
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            k[kk] = *(const u32x4*)(stage[buf] + chunk_at<D / 8>(32 * kt + n, frag_dim(kk >> 1, kk & 1, hf) / 8));
-          half_score[kt] = qf.score(k);
+          for (int kt = 0; kt < TILE_KEYS / 32; ++kt) {
+            u32x4 k[D / 16];
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+              k[kk] = *(const u32x4*)(stage[buf] + chunk_at<D / 8>(32 * kt + n, frag_dim(kk >> 1, kk & 1, hf) / 8));
+            half_score[kt] = qf.score(k, hf);
+          }
+          float s = hf ? half_score[1] : half_score[0];
+          if (FP8) s *= key_scale[buf][lane];
+          const int j = base + lane;
+          if (j < my_thr && j < hi) out[j] = key_ok[buf][lane] ? kept_score(s) : SEL_NONE;
         }
-        float s = hf ? half_score[1] : half_score[0];
-        if (FP8) s *= key_scale[buf][lane];
-        const int j = base + lane;
-        if (j < my_thr && j < hi) out[j] = key_ok[buf][lane] ? kept_score(s) : SEL_NONE;
+        if (base + TILE_KEYS < hi) put(buf ^ 1);
+        __syncthreads();
       }
-      if (more) put(buf ^ 1);
-      __syncthreads();
     }
     if (norms) {
 #pragma unroll
