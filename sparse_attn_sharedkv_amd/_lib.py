@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -124,6 +125,21 @@ class SasSelectArgs(ctypes.Structure):
                                                "table_len", "max_keys", "dtype", "key_format")])
 
 
+def packer(cls):
+    """``struct.Struct.pack`` for the fields of ``cls`` in order: the bytes of one call's arguments.
+
+    A call's arguments are packed in one step because setting 25 fields of a ctypes structure one
+    by one costs several microseconds, as much as the smallest kernels take.
+    """
+    codes = {ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_float: "f"}
+    layout = struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_) + "0P")
+    assert layout.size == ctypes.sizeof(cls)
+    return layout.pack
+
+
+pack_row_args = packer(SasRowArgs)
+pack_select_args = packer(SasSelectArgs)
+
 EXPORTS = ("sas_metadata_build", "sas_metadata_build_device", "sas_metadata_build_device_cu",
            "sas_workspace_bytes", "sas_attention_launch", "sas_attention_launch_lens",
            "sas_attention_launch_noalloc", "sas_merge_sync_take", "sas_kv_fp8_append",
@@ -176,11 +192,11 @@ def load() -> ctypes.CDLL:
                                           ctypes.c_int, ctypes.c_int64, ctypes.c_void_p]
         for entry in (lib.sas_norm_rope, lib.sas_kv_append_rope):
             entry.restype = ctypes.c_int
-            entry.argtypes = [ctypes.POINTER(SasRowArgs), ctypes.c_void_p]
+            entry.argtypes = [ctypes.c_void_p, ctypes.c_void_p]  # (packed arguments or byref)
         lib.sas_topk_select.restype = ctypes.c_int
-        lib.sas_topk_select.argtypes = [ctypes.POINTER(SasSelectArgs), ctypes.c_void_p]
+        lib.sas_topk_select.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
         lib.sas_topk_select_workspace.restype = ctypes.c_int64
-        lib.sas_topk_select_workspace.argtypes = [ctypes.POINTER(SasSelectArgs)]
+        lib.sas_topk_select_workspace.argtypes = [ctypes.c_void_p]
         lib.sas_row_args_struct_size.restype = ctypes.c_int
         lib.sas_select_args_struct_size.restype = ctypes.c_int
         lib.sas_version.restype = ctypes.c_int

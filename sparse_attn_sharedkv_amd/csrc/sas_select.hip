@@ -562,16 +562,16 @@ __global__ __launch_bounds__(64 * TILE_WAVES) void score_tile_kernel(SasSelectAr
         if (active) {
           // both halves of the stage without a branch between them, so that one's weighted sums
           // can run under the other's products; then each half of the wave keeps 32 scores
-          float half_score[2];
-#pragma unroll
+          float s = 0.0f;
+#pragma unroll(MT *D <= 256 ? TILE_KEYS / 32 : 1)
           for (int kt = 0; kt < TILE_KEYS / 32; ++kt) {
             u32x4 k[D / 16];
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk)
               k[kk] = *(const u32x4*)(stage[buf] + chunk_at<D / 8>(32 * kt + n, frag_dim(kk >> 1, kk & 1, hf) / 8));
-            half_score[kt] = qf.score(k, hf);
+            const float part = qf.score(k, hf);
+            s = hf == kt ? part : s;
           }
-          float s = hf ? half_score[1] : half_score[0];
           if (FP8) s *= key_scale[buf][lane];
           const int j = base + lane;
           if (j < my_thr && j < hi) out[j] = key_ok[buf][lane] ? kept_score(s) : SEL_NONE;
@@ -818,7 +818,7 @@ __device__ inline void find_bin(int need, SelSlot slot, SelShared<THREADS>& sh) 
   __syncthreads();
 }
 
-// A monotone map of [lo, hi] onto the bins (values outside go below bin 0, or to the last).
+// A monotone map of [lo, hi] onto the bins.
 template <int THREADS>
 struct BinMap {
   float base, inv;
@@ -826,11 +826,9 @@ struct BinMap {
     return {0.5f * lo, (float)(SelSize<THREADS>::BINS - 1) / (0.5f * hi - 0.5f * lo)};
   }
   __device__ bool usable() const { return inv < SEL_MAX; }
+  // lo <= x <= hi: 0.5 x - base is in [0, 0.5 hi - base], its product below BINS
+  __device__ int bin(float x) const { return (int)(fmaf(0.5f, x, -base) * inv); }
   __device__ float edge(int bin) const { return 2.0f * ((float)bin / inv + base); }  // about
-  __device__ int bin(float x) const {
-    const float b = fminf((0.5f * x - base) * inv, (float)(SelSize<THREADS>::BINS - 1));
-    return b < 0.0f ? -1 : (int)b;
-  }
 };
 
 // The choice from scores in memory, for what the registers and lists do not hold.
@@ -914,7 +912,7 @@ __device__ inline void select_from_memory(const SasSelectArgs& a, const SelPlan&
   while (lo < hi) {
     const BinMap<THREADS> map = BinMap<THREADS>::of(lo, hi);
     if (!map.usable()) break;
-    auto bin_of = [&](float x) { return max(map.bin(x), 0); };
+    auto bin_of = [&](float x) { return map.bin(x); };
     __syncthreads();
     for (int i = tid; i < BINS; i += THREADS) sh.bins[i] = 0;
     if (tid == 0) sh.count = 0;
@@ -1010,41 +1008,55 @@ __device__ inline void select_from_memory(const SasSelectArgs& a, const SelPlan&
     return;
   }
   // more of them than the list holds (equal keys, or a bound that is not finite): the rest-th
-  // largest 64-bit score by its bytes, the scores formed again for each
+  // largest 64-bit score digit by digit. A row whose digits so far are not those of that score is
+  // marked taken or not and is not scored again, so the most rows are scored two or three times.
+  constexpr int DIGIT = THREADS == 64 ? 9 : THREADS == 256 ? 10 : 11;  // 2^DIGIT bins
+  const float tie_x = SEL_MAX;
   uint64_t prefix = 0;
   int want = rest;
-  for (int shift = 56; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += THREADS) sh.bins[i] = 0;
+  for (int j = tid; j < n; j += THREADS) {
+    const float x = x_of[j];
+    if (x > b_hi) {
+      x_of[j] = taken_x;
+    } else if (!(x >= b_lo) || x == SEL_NONE) {
+      x_of[j] = SEL_NONE;
+    } else {
+      x_of[j] = tie_x;  // (as far as is known)
+    }
+  }
+  for (int seen = 0; seen < 64; seen += DIGIT) {
+    const int left = 64 - seen, digit_bits = left < DIGIT ? left : DIGIT, shift = left - digit_bits;
+    for (int i = tid; i < BINS; i += THREADS) sh.bins[i] = 0;
     __syncthreads();
     for (int j0 = 16 * wave; j0 < n; j0 += 16 * WAVES) {
       const int j = min(j0 + (lane & 15), n - 1);
-      const float x = x_of[j];
-      const bool in = x >= b_lo && x <= b_hi && x != SEL_NONE && j0 + (lane & 15) < n;
-      if (!__any(in)) continue;
+      const bool tied = x_of[j] == tie_x;
+      if (!__any(tied)) continue;
       const uint64_t key = order64<T, FP8>(a, p, t, table, j, lane);
-      if (lane < 16 && in && (shift == 56 || key >> (shift + 8) == prefix))
-        atomicAdd(&sh.bins[(key >> shift) & 255], 1u);
+      if (lane < 16 && tied && j0 + lane < n) {
+        const uint64_t head = seen == 0 ? 0 : key >> left;
+        if (head == prefix) {
+          atomicAdd(&sh.bins[(key >> shift) & ((1u << digit_bits) - 1)], 1u);
+        } else {
+          x_of[j] = head > prefix ? taken_x : SEL_NONE;
+        }
+      }
     }
     __syncthreads();
-    int digit = 255, above = 0;
-    while (digit > 0 && above + (int)sh.bins[digit] < want) above += (int)sh.bins[digit--];
-    want -= above;
-    prefix = (prefix << 8) | (uint64_t)digit;
+    find_bin<THREADS>(want, SLOT_COUNT, sh);
+    want -= sh.below;
+    prefix = (prefix << digit_bits) | (uint64_t)sh.found;
     __syncthreads();
   }
   for (int j0 = 16 * wave; j0 < n; j0 += 16 * WAVES) {
     const int j = min(j0 + (lane & 15), n - 1);
-    const float x = x_of[j];
-    float y = x > b_hi ? taken_x : SEL_NONE;
-    const bool in = x >= b_lo && x <= b_hi && x != SEL_NONE;
-    if (__any(in)) {
-      const uint64_t key = order64<T, FP8>(a, p, t, table, j, lane);
-      if (in) y = key > prefix ? taken_x : key == prefix ? SEL_MAX : SEL_NONE;
-    }
-    if (lane < 16 && j0 + lane < n) x_of[j] = y;
+    const bool tied = x_of[j] == tie_x;
+    if (!__any(tied)) continue;
+    const uint64_t key = order64<T, FP8>(a, p, t, table, j, lane);
+    if (lane < 16 && tied && j0 + lane < n && key != prefix) x_of[j] = key > prefix ? taken_x : SEL_NONE;
   }
   __syncthreads();
-  emit([&](int j) { return x_of[j] > SEL_MAX; }, [&](int j) { return x_of[j] == SEL_MAX; }, want);
+  emit([&](int j) { return x_of[j] > SEL_MAX; }, [&](int j) { return x_of[j] == tie_x; }, want);
 }
 
 // Rows longer than this have no place in the map of select_kernel's ids.
@@ -1284,36 +1296,12 @@ __global__ __launch_bounds__(THREADS, THREADS == 64 ? 5 : 4) void select_kernel(
       for (int round = 0;; ++round) {
         m = BinMap<THREADS>::of(lo, hi);
         if (!(lo < hi) || !m.usable() || round == 4) return false;
-        // (of many values per thread only those above a bin that a sample of them puts a
-        // little below the topk-th are counted, by the rule of the list's sample)
-        int floor_bin = 0;
-        if (VPT >= 16 && THREADS == 1024 && runs >= 4 && round == 0) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (x[i] != SEL_NONE) atomicAdd(&sh.bins[m.bin(x[i])], 1u);
-          }
-          const float share = (float)k * (4.0f * THREADS) / (float)n;
-          __syncthreads();
-          find_bin<THREADS>((int)(share + 6.0f * sqrtf(2.0f * share) + 8.0f), SLOT_SAMPLE, sh);
-          floor_bin = sh.found;
-          for (int i = tid; i < BINS; i += THREADS) sh.bins[i] = 0;
-          __syncthreads();
+        for (int i = 0; i < VPT; ++i) {
+          if (x[i] >= lo && x[i] <= hi) atomicAdd(&sh.bins[m.bin(x[i])], 1u);
         }
-        auto count = [&](int from, int to) {
-#pragma unroll
-          for (int i = 0; i < VPT; ++i) {
-            const int b = m.bin(x[i]);
-            if (x[i] >= lo && x[i] <= hi && b >= from && b < to) atomicAdd(&sh.bins[b], 1u);
-          }
-          if (tid == 0) sh.found = -1;
-          __syncthreads();
-          find_bin<THREADS>(need, SLOT_COUNT, sh);
-        };
-        count(floor_bin, BINS);
-        if (sh.found < 0) {  // (the sample put it too high: the others are counted too)
-          __syncthreads();
-          count(0, floor_bin);
-        }
+        __syncthreads();
+        find_bin<THREADS>(need, SLOT_COUNT, sh);
         bin = sh.found;
         need -= sh.below;
         if (sh.in_bin <= LIST / 2) break;

@@ -20,7 +20,6 @@ rows, their ``block_size * D`` e4m3 codes and behind those their fp32 scales, on
 
 from __future__ import annotations
 
-import ctypes
 from typing import Optional, Tuple
 
 import torch
@@ -34,84 +33,101 @@ INDEX_DIMS = (64, 128)
 
 def no_grad_inputs(who: str, *tensors) -> None:
     """Refuse inputs whose gradient the caller would silently not get."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{who} has no backward pass: call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{who} has no backward pass: call it under torch.no_grad()")
 
 
-def launch_on(dev: torch.device, entry, args) -> None:
-    """Enqueue a library call on the current stream of ``dev``."""
-    if torch.cuda.current_device() == dev.index:
-        rc = entry(ctypes.byref(args), torch.cuda.current_stream(dev).cuda_stream)
+def launch_on(index: int, entry, packed: bytes) -> None:
+    """Enqueue a library call on the current stream of GPU ``index``."""
+    # (the raw handle: torch.cuda.current_stream makes an object first, 1.5 us of a 10 us call)
+    if torch.cuda.current_device() == index:
+        rc = entry(packed, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(dev):
-            rc = entry(ctypes.byref(args), torch.cuda.current_stream(dev).cuda_stream)
+        with torch.cuda.device(index):
+            rc = entry(packed, torch._C._cuda_getCurrentRawStream(index))
     if rc != _lib.SAS_OK:
         raise RuntimeError(_lib.last_error())
 
 
-def _device_int32(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+def device_int32(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """``t`` as contiguous int32 on ``dev``: itself where it is that already."""
     if t.dtype != torch.int32 or t.device != dev:
         t = t.to(device=dev, dtype=torch.int32)
-    return t.reshape(-1).contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _common(who: str, x: torch.Tensor, tokens: int, positions: Optional[torch.Tensor],
-            cos_sin: Optional[torch.Tensor], norm_weight: Optional[torch.Tensor], norm_eps: float,
-            rope_offset: Optional[int], interleaved: bool) -> Tuple[_lib.SasRowArgs, list]:
-    """The arguments both calls share, checked, and the tensors behind their pointers."""
+def _common(who, x, d, tokens, positions, cos_sin, norm_weight, norm_eps, rope_offset, interleaved):
+    """The arguments both calls share, checked.
+
+    Returns the tensors behind the pointers (kept alive until the launch) and the values of
+    ``SasRowArgs`` that follow from them: (positions, cos_sin, norm_weight pointers), (norm_dim,
+    rope_dim, rope_offset, interleaved, max_position, dtype, norm_weight_fp32), eps.
+    """
     no_grad_inputs(who, x, cos_sin, norm_weight)
-    d, dev = x.shape[-1], x.device
-    if x.dtype not in _DTYPES:
-        raise ValueError(f"{who}: rows must be bf16 or fp16 (got {x.dtype})")
+    dtype, dev = x.dtype, x.device
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise ValueError(f"{who}: rows must be bf16 or fp16 (got {dtype})")
     if d % 8 or not 8 <= d <= _lib.ROW_MAX_DIM:
         raise ValueError(f"{who}: the row width must be a multiple of 8 up to {_lib.ROW_MAX_DIM} "
                          f"(got {d})")
-    a = _lib.SasRowArgs()
-    keep = []
-    a.tokens, a.dim, a.dtype, a.eps = tokens, d, _DTYPES[x.dtype], norm_eps
-    a.interleaved = int(bool(interleaved))
+    p_pos = p_cos = p_w = n = r = off = table = w_fp32 = 0
     if norm_weight is not None:
         n = norm_weight.numel()
         if norm_weight.dim() != 1 or n % 8 or not 8 <= n <= d:
             raise ValueError(f"{who}: norm_weight must have a multiple of 8 entries up to the row "
                              f"width {d} (got {tuple(norm_weight.shape)})")
-        if norm_weight.dtype not in (torch.float32, x.dtype):
+        w_fp32 = int(norm_weight.dtype == torch.float32)
+        if not w_fp32 and norm_weight.dtype != dtype:
             raise ValueError(f"{who}: norm_weight must be fp32 or the rows' type")
         if norm_weight.device != dev:
             raise ValueError(f"{who}: all tensors must be on the rows' device")
-        norm_weight = _aligned(norm_weight.contiguous())
-        a.norm_weight, a.norm_dim = norm_weight.data_ptr(), n
-        a.norm_weight_fp32 = int(norm_weight.dtype == torch.float32)
-        keep.append(norm_weight)
+        norm_weight = _plain(norm_weight)
+        p_w = norm_weight.data_ptr()
     if (cos_sin is None) != (positions is None):
         raise ValueError(f"{who}: positions and cos_sin belong together")
     if cos_sin is not None:
         if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32 or cos_sin.shape[0] < 1:
             raise ValueError(f"{who}: cos_sin must be fp32 [positions, rotated dims]")
-        r = cos_sin.shape[1]
+        table, r = cos_sin.shape
         off = d - r if rope_offset is None else int(rope_offset)
         if r % (8 if interleaved else 16) or r < 8 or off % 8 or off < 0 or off + r > d:
             raise ValueError(
                 f"{who}: cannot rotate dims [{off}, {off + r}) of {d}: the offset must be a multiple "
                 "of 8 and their number of 8 (interleaved pairs) or 16 (halves)")
+        if table >= 1 << 31:
+            raise ValueError(f"{who}: 2^31 positions or more")
         if positions.numel() != tokens:
             raise ValueError(f"{who}: positions must have one entry for each of {tokens} rows "
                              f"(got {positions.numel()})")
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"{who}: positions must be int32 or int64")
         if cos_sin.device != dev:
             raise ValueError(f"{who}: all tensors must be on the rows' device")
-        cos_sin = _aligned(cos_sin.contiguous())
-        positions = _device_int32(positions, dev) if dev.type == "cuda" else positions
-        a.positions, a.cos_sin = positions.data_ptr(), cos_sin.data_ptr()
-        a.max_position, a.rope_dim, a.rope_offset = cos_sin.shape[0], r, off
-        keep += [positions, cos_sin]
+        if x.is_cuda:
+            if positions.dtype == torch.int64:
+                positions = _narrow(positions)
+            positions = device_int32(positions, dev)
+        cos_sin = _plain(cos_sin)
+        p_pos, p_cos = positions.data_ptr(), cos_sin.data_ptr()
     elif rope_offset is not None:
         raise ValueError(f"{who}: rope_offset without cos_sin")
-    return a, keep
+    return ((positions, cos_sin, norm_weight), (p_pos, p_cos, p_w),
+            (n, r, off, 1 if interleaved else 0, table, code, w_fp32), norm_eps)
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """``t`` or a copy of it that starts on 16 bytes."""
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+def _plain(t: torch.Tensor) -> torch.Tensor:
+    """``t`` or a contiguous copy of it that starts on 16 bytes."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _narrow(t: torch.Tensor) -> torch.Tensor:
+    """int64 places inside int32: one past it stays out of range instead of coming back inside."""
+    return t.clamp(-1, (1 << 31) - 1)
 
 
 def norm_rope_heads(q: torch.Tensor, *, positions: Optional[torch.Tensor] = None,
@@ -130,61 +146,73 @@ def norm_rope_heads(q: torch.Tensor, *, positions: Optional[torch.Tensor] = None
     goes (``q`` itself is allowed: dims that nothing changes are then not touched).
     """
     who = "norm_rope_heads"
-    if q.dim() < 2:
-        raise ValueError(f"{who}: q must be [..., heads, head dim] (got {tuple(q.shape)})")
-    h, d = q.shape[-2], q.shape[-1]
+    shape = q.shape
+    if len(shape) < 2:
+        raise ValueError(f"{who}: q must be [..., heads, head dim] (got {tuple(shape)})")
+    h, d = shape[-2], shape[-1]
     if h < 1:
         raise ValueError(f"{who}: q has no heads")
     tokens = q.numel() // (h * d) if d else 0
-    a, keep = _common(who, q, tokens, positions, cos_sin, norm_weight, norm_eps, rope_offset,
-                      interleaved)
+    keep, pointers, (n, r, off, *rest), eps = _common(
+        who, q, d, tokens, positions, cos_sin, norm_weight, norm_eps, rope_offset, interleaved)
     if tokens * h >= 1 << 31:
         raise ValueError(f"{who}: 2^31 heads or more in one call")
     if out is not None:
         no_grad_inputs(who, out)
-        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+        if out.shape != shape or out.dtype != q.dtype or out.device != q.device:
             raise ValueError(f"{who}: out must have q's shape, type and device")
-    if q.device.type != "cuda":
+    if not q.is_cuda:
         raise RuntimeError(f"{who} runs on a ROCm GPU; q is on {q.device}")
+    x = _token_view(q, h, d)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    x, y = _token_view(q, h, d), _token_view(out, h, d)
-    if y is None:
-        raise ValueError(f"{who}: out must have heads of contiguous dims aligned to 16 bytes, its "
-                         "tokens one stride apart")
-    if x is None:
-        x = q.reshape(tokens, h, d).contiguous()
-        x = _aligned(x)
-    elif x.data_ptr() != y.data_ptr() or x.stride() != y.stride():
-        _no_overlap(who, x, y)
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        y = (out.data_ptr(), h * d, d)
+        if x is None:
+            q = _plain(q)
+            x = (q.data_ptr(), h * d, d)
+    else:
+        y = _token_view(out, h, d)
+        if y is None:
+            raise ValueError(f"{who}: out must have heads of contiguous dims aligned to 16 bytes, "
+                             "its tokens one stride apart")
+        if x is None:
+            _no_overlap(who, q, out)
+            q = _plain(q)
+            x = (q.data_ptr(), h * d, d)
+        elif x != y:
+            _no_overlap(who, q, out)
     if tokens == 0:
         return out
-    a.heads = h
-    if x.data_ptr() == y.data_ptr() and not a.norm_dim:
+    skip = 0
+    if x == y and not n:
         # in place: only the rotated dims are read and written
-        if not a.rope_dim:
+        if not r:
             return out
-        x = y = x[..., a.rope_offset:a.rope_offset + a.rope_dim]
-        a.dim, a.rope_offset = a.rope_dim, 0
-    a.x, a.out = x.data_ptr(), y.data_ptr()
-    a.x_token_stride, a.x_head_stride = x.stride(0), x.stride(1)
-    a.out_token_stride, a.out_head_stride = y.stride(0), y.stride(1)
-    launch_on(q.device, _lib.load().sas_norm_rope, a)
+        skip, d, off = 2 * off, r, 0
+    packed = _lib.pack_row_args(x[0] + skip, y[0] + skip, *pointers, 0, x[1], x[2], y[1], y[2], 0,
+                                tokens, h, d, n, r, off, *rest, 0, 0, eps, 0)
+    launch_on(q.get_device(), _lib.load().sas_norm_rope, packed)
     del keep
     return out
 
 
-def _token_view(t: torch.Tensor, h: int, d: int) -> Optional[torch.Tensor]:
-    """``t`` as ``[tokens, h, d]`` without a copy, as the kernel can read it, or None."""
-    try:
-        v = t if t.dim() == 3 else t.view(-1, h, d)
-    except RuntimeError:
+def _token_view(t: torch.Tensor, h: int, d: int) -> Optional[Tuple[int, int, int]]:
+    """(address, token stride, head stride) of ``t`` as ``[tokens, h, d]`` as the kernel can read
+    it, or None."""
+    at = t.data_ptr()
+    if at % 16:
         return None
-    if d > 1 and v.stride(2) != 1 or v.data_ptr() % 16:
+    if t.is_contiguous():
+        return at, h * d, d
+    if t.dim() != 3:
+        try:
+            t = t.view(-1, h, d)
+        except RuntimeError:
+            return None
+    tokens, heads, dims = t.stride()
+    if dims != 1 or (t.shape[0] > 1 and tokens % 8) or (h > 1 and heads % 8):
         return None
-    if v.shape[0] > 1 and v.stride(0) % 8 or h > 1 and v.stride(1) % 8:
-        return None
-    return v
+    return at, tokens - tokens % 8, heads - heads % 8  # (strides of one are not used)
 
 
 def _no_overlap(who: str, x: torch.Tensor, y: torch.Tensor) -> None:
@@ -218,22 +246,25 @@ def append_kv_rope(cache: torch.Tensor, kv: torch.Tensor, slot_mapping: torch.Te
     cache's device.
     """
     who = "append_kv_rope"
-    if kv.dim() not in (2, 3) or (kv.dim() == 3 and kv.shape[1] != 1):
-        raise ValueError(f"{who}: kv must be [n, D] or [n, 1, D] (got {tuple(kv.shape)})")
-    n, d = kv.shape[0], kv.shape[-1]
-    a, keep = _common(who, kv, n, positions, cos_sin, norm_weight, norm_eps, rope_offset,
-                      interleaved)
+    shape = kv.shape
+    if len(shape) not in (2, 3) or (len(shape) == 3 and shape[1] != 1):
+        raise ValueError(f"{who}: kv must be [n, D] or [n, 1, D] (got {tuple(shape)})")
+    n_rows, d = shape[0], shape[-1]
+    keep, pointers, (n, r, off, *rest), eps = _common(
+        who, kv, d, n_rows, positions, cos_sin, norm_weight, norm_eps, rope_offset, interleaved)
     if cache.dim() != 4 or cache.shape[2] != 1:
         raise ValueError(f"{who}: cache must be [blocks, block_size, 1, width] "
                          f"(got {tuple(cache.shape)})")
     if not cache.is_contiguous():
         raise ValueError(f"{who}: cache must be contiguous (it is written in place)")
     blocks, block_size, _, width = cache.shape
-    if cache.dtype in _FP8_TYPES:
+    dtype = cache.dtype
+    row_format = _lib.ROW_NATIVE
+    if dtype in _FP8_TYPES:
         if width == _lib.FP8_ROW_BYTES and d == 576 and kv.dtype == torch.bfloat16:
-            a.row_format = _lib.ROW_FP8_DS_MLA
+            row_format = _lib.ROW_FP8_DS_MLA
         elif width == d + 4 and d in INDEX_DIMS:
-            a.row_format = _lib.ROW_FP8_INDEX
+            row_format = _lib.ROW_FP8_INDEX
             if block_size * width % 16:
                 raise ValueError(f"{who}: fp8 index pages must be a multiple of 16 bytes "
                                  f"(block_size {block_size})")
@@ -241,31 +272,33 @@ def append_kv_rope(cache: torch.Tensor, kv: torch.Tensor, slot_mapping: torch.Te
             raise ValueError(f"{who}: an fp8 cache has rows of {_lib.FP8_ROW_BYTES} bytes for 576 "
                              f"bf16 dims, or of D + 4 for D in {INDEX_DIMS} (got width {width} for "
                              f"{d} dims of {kv.dtype})")
-    elif cache.dtype != kv.dtype or width != d:
-        raise ValueError(f"{who}: a native cache has kv's type and width (got {cache.dtype} of "
+    elif dtype != kv.dtype or width != d:
+        raise ValueError(f"{who}: a native cache has kv's type and width (got {dtype} of "
                          f"{width} for {kv.dtype} of {d})")
-    if slot_mapping.numel() != n:
+    if slot_mapping.numel() != n_rows:
         raise ValueError(f"{who}: slot_mapping must have one entry per kv row")
     if slot_mapping.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{who}: slot_mapping must be int32 or int64")
-    if blocks * block_size >= 1 << 31:
+    cache_rows = blocks * block_size
+    if cache_rows >= 1 << 31:
         raise ValueError(f"{who}: 2^31 cache rows or more")
-    if cache.device.type != "cuda" or kv.device != cache.device:
+    dev = cache.device
+    if not cache.is_cuda or kv.device != dev:
         raise RuntimeError(f"{who} runs on a ROCm GPU; cache and kv must share it")
-    if cache.data_ptr() % 16:
+    at = cache.data_ptr()
+    if at % 16:
         raise ValueError(f"{who}: cache must be aligned to 16 bytes")
-    if n == 0 or cache.numel() == 0:
+    if n_rows == 0 or cache_rows == 0:
         return
-    rows = kv.reshape(n, d) if kv.dim() == 3 else kv
-    if (rows.stride(1) != 1 or (n > 1 and rows.stride(0) % 8) or rows.data_ptr() % 16):
-        rows = _aligned(rows.contiguous())
+    stride = kv.stride(0)
+    if kv.stride(-1) != 1 or stride % 8 or kv.data_ptr() % 16:
+        kv = _plain(kv)
+        stride = d
     if slot_mapping.dtype == torch.int64:
-        # (a slot past int32 is past the pool; narrowing alone could bring it back inside)
-        slot_mapping = slot_mapping.clamp(-1, (1 << 31) - 1)
-    slots = _device_int32(slot_mapping, cache.device)
-    keep += [rows, slots]
-    a.heads, a.x, a.out, a.slots = 1, rows.data_ptr(), cache.data_ptr(), slots.data_ptr()
-    a.x_token_stride = rows.stride(0)
-    a.cache_rows, a.block_size = blocks * block_size, block_size
-    launch_on(cache.device, _lib.load().sas_kv_append_rope, a)
+        slot_mapping = _narrow(slot_mapping)
+    slots = device_int32(slot_mapping, dev)
+    packed = _lib.pack_row_args(kv.data_ptr(), at, *pointers, slots.data_ptr(), stride, 0, 0, 0,
+                                cache_rows, n_rows, 1, d, n, r, off, *rest, row_format, block_size,
+                                eps, 0)
+    launch_on(cache.get_device(), _lib.load().sas_kv_append_rope, packed)
     del keep

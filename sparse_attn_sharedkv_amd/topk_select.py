@@ -8,13 +8,22 @@ ids of the best ``topk`` come back in the form the attention takes. No reference
 
 from __future__ import annotations
 
-import ctypes
+import functools
 from typing import Optional
 
 import torch
 
 from . import _lib
-from .rows import _DTYPES, _FP8_TYPES, INDEX_DIMS, _aligned, launch_on, no_grad_inputs
+from .rows import _DTYPES, _FP8_TYPES, INDEX_DIMS, _plain, device_int32, launch_on, no_grad_inputs
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(sizes: tuple) -> int:
+    """Workspace of a call with these sizes (the int32 fields of ``SasSelectArgs``)."""
+    need = _lib.load().sas_topk_select_workspace(_lib.pack_select_args(*[0] * 9, *sizes))
+    if need < 0:
+        raise RuntimeError(_lib.last_error())
+    return need
 
 
 def sparse_topk_indices(q_index: torch.Tensor, *, weights: torch.Tensor, index_k: torch.Tensor,
@@ -107,37 +116,28 @@ def sparse_topk_indices(q_index: torch.Tensor, *, weights: torch.Tensor, index_k
         raise ValueError("too many query rows in one call")
 
     dev = q_index.device
-    if dev.type != "cuda":
+    if not q_index.is_cuda:
         raise RuntimeError("sparse_topk_indices runs on a ROCm GPU; q_index is on " + str(dev))
     if index_k.device != dev or weights.device != dev:
         raise ValueError("all tensors must be on q_index's device")
     i32 = torch.int32
-    q = _aligned(q_index.contiguous())
-    keys = _aligned(index_k.contiguous())
-    w = weights.to(torch.float32).contiguous()
-    table = index_block_table.to(device=dev, dtype=i32).contiguous()
-    lens = seqused_kv.to(device=dev, dtype=i32).contiguous()
-    cu = None if cu_seqlens_q is None else cu_seqlens_q.to(device=dev, dtype=i32).contiguous()
+    q, keys = _plain(q_index), _plain(index_k)
+    w = weights if weights.dtype == torch.float32 else weights.float()
+    if not w.is_contiguous():
+        w = w.contiguous()
+    table, lens = device_int32(index_block_table, dev), device_int32(seqused_kv, dev)
+    cu = None if cu_seqlens_q is None else device_int32(cu_seqlens_q, dev)
     out = torch.empty((*q_index.shape[:-2], 1, k), dtype=i32, device=dev)
     if total == 0:
         return out
     if nb == 0:
         return out.fill_(-1)
-
-    a = _lib.SasSelectArgs()
-    a.q, a.weights, a.keys = q.data_ptr(), w.data_ptr(), keys.data_ptr()
-    a.block_table, a.seqused_kv, a.out = table.data_ptr(), lens.data_ptr(), out.data_ptr()
-    a.cu_seqlens_q = None if cu is None else cu.data_ptr()
-    a.batch, a.tokens, a.rows_per_seq = nb, total, rows_per_seq
-    a.heads, a.dim, a.topk, a.cmp_ratio = h, d, k, ratio
-    a.block_num, a.block_size, a.table_len = blocks, block_size, table.shape[1]
-    a.max_keys, a.dtype = max_keys, _DTYPES[dtype]
-    a.key_format = _lib.ROW_FP8_INDEX if fp8 else _lib.ROW_NATIVE
-    lib = _lib.load()
-    need = lib.sas_topk_select_workspace(ctypes.byref(a))
-    if need < 0:
-        raise RuntimeError(_lib.last_error())
+    sizes = (nb, total, rows_per_seq, h, d, k, ratio, blocks, block_size, table.shape[1], max_keys,
+             _DTYPES[dtype], _lib.ROW_FP8_INDEX if fp8 else _lib.ROW_NATIVE)
+    need = _workspace_bytes(sizes)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), need
-    launch_on(dev, lib.sas_topk_select, a)
+    packed = _lib.pack_select_args(q.data_ptr(), w.data_ptr(), keys.data_ptr(), table.data_ptr(),
+                                   0 if cu is None else cu.data_ptr(), lens.data_ptr(),
+                                   out.data_ptr(), ws.data_ptr(), need, *sizes)
+    launch_on(q_index.get_device(), _lib.load().sas_topk_select, packed)
     return out
