@@ -7,7 +7,10 @@
 // and then the pairs of dims [off, off + R) are turned by the angle of the row's position:
 //   (a, b) -> (a cos - b sin, b cos + a sin)
 // with pair i = dims (2i, 2i + 1) of the range (interleaved) or (i, i + R / 2) (halves), and
-// cos / sin from the caller's fp32 table. Everything is in fp32 and rounded once, at the store.
+// cos / sin from the caller's fp32 table. Everything is in fp32 and rounded once, at the store; rows
+// that end in fp8 are in 64 bits up to the value that is quantized, which a code's coarse steps
+// would otherwise turn an fp32 rounding of into a whole step (16384 rows: no slower, the rows'
+// bytes decide).
 //
 // Bound by memory: a row is read once and written once. A group of G lanes (8 to 64, the fewest
 // that hold the row at 16 bytes a lane, two or four loads a lane above 512 dims) owns a row, so
@@ -37,27 +40,41 @@ struct Vec8 {
   typedef T type __attribute__((ext_vector_type(8)));
 };
 
-template <typename T>
-__device__ inline void load8(const void* p, float f[8]) {
+template <typename T, typename W>
+__device__ inline void load8(const void* p, W f[8]) {
   const typename Vec8<T>::type v = *(const typename Vec8<T>::type*)p;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = (float)v[i];
+  for (int i = 0; i < 8; ++i) f[i] = (W)(float)v[i];
 }
 
-__device__ inline void load8f(const float* p, float f[8]) {
+template <typename W>
+__device__ inline void load8f(const float* p, W f[8]) {
   const float4 a = ((const float4*)p)[0], b = ((const float4*)p)[1];
   f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
   f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
 }
 
-template <typename T>
-__device__ inline void norm_weight8(const SasRowArgs& a, int e0, float w[8]) {
+template <typename T, typename W>
+__device__ inline void norm_weight8(const SasRowArgs& a, int e0, W w[8]) {
   if (a.norm_weight_fp32) {
     load8f((const float*)a.norm_weight + e0, w);
   } else {
     load8<T>((const T*)a.norm_weight + e0, w);
   }
 }
+
+template <int OUT>
+struct WideOf {
+  typedef float type;
+};
+template <>
+struct WideOf<OUT_FP8_MLA> {
+  typedef double type;
+};
+template <>
+struct WideOf<OUT_FP8_INDEX> {
+  typedef double type;
+};
 
 template <typename T, int G, int NCH, int OUT>
 __global__ __launch_bounds__(ROWS_WG) void rows_kernel(SasRowArgs a) {
@@ -74,7 +91,8 @@ __global__ __launch_bounds__(ROWS_WG) void rows_kernel(SasRowArgs a) {
   const T* x = (const T*)a.x + (int64_t)t * a.x_token_stride + (int64_t)h * a.x_head_stride;
   const int chunks = a.dim >> 3;
 
-  float f[NCH][8];
+  typedef typename WideOf<OUT>::type W;
+  W f[NCH][8];
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
     const int c = lane + i * G;
@@ -82,12 +100,12 @@ __global__ __launch_bounds__(ROWS_WG) void rows_kernel(SasRowArgs a) {
       load8<T>(x + 8 * c, f[i]);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[i][e] = 0.0f;
+      for (int e = 0; e < 8; ++e) f[i][e] = 0;
     }
   }
   // the other members of the halves' pairs, before anything is stored
   const int r0 = a.rope_offset, r1 = r0 + a.rope_dim, half = a.rope_dim >> 1;
-  float p[NCH][8];
+  W p[NCH][8];
   if (!a.interleaved) {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
@@ -97,21 +115,21 @@ __global__ __launch_bounds__(ROWS_WG) void rows_kernel(SasRowArgs a) {
   }
 
   if (a.norm_dim > 0) {
-    float s = 0.0f;
+    W s = 0;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       if (8 * (lane + i * G) < a.norm_dim) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s = fmaf(f[i][e], f[i][e], s);
+        for (int e = 0; e < 8; ++e) s = fma(f[i][e], f[i][e], s);
       }
     }
 #pragma unroll
     for (int off = 1; off < G; off <<= 1) s += __shfl_xor(s, off, 64);
-    const float inv = 1.0f / sqrtf(s / (float)a.norm_dim + a.eps);
+    const W inv = (W)1 / sqrt(s / (W)a.norm_dim + (W)a.eps);
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
       const int e0 = 8 * (lane + i * G);
-      float w[8];
+      W w[8];
       if (e0 < a.norm_dim) {
         norm_weight8<T>(a, e0, w);
 #pragma unroll
@@ -136,7 +154,7 @@ __global__ __launch_bounds__(ROWS_WG) void rows_kernel(SasRowArgs a) {
     for (int i = 0; i < NCH; ++i) {
       const int e0 = 8 * (lane + i * G);
       if (e0 < r0 || e0 >= r1) continue;
-      float c[8], s[8];
+      W c[8], s[8];
       if (a.interleaved) {
         const float4 cv = *(const float4*)(cs + ((e0 - r0) >> 1));
         const float4 sv = *(const float4*)(cs + half + ((e0 - r0) >> 1));
@@ -144,7 +162,7 @@ __global__ __launch_bounds__(ROWS_WG) void rows_kernel(SasRowArgs a) {
         s[0] = sv.x, s[1] = sv.y, s[2] = sv.z, s[3] = sv.w;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float u = f[i][2 * j], v = f[i][2 * j + 1];
+          const W u = f[i][2 * j], v = f[i][2 * j + 1];
           f[i][2 * j] = u * c[j] - v * s[j];
           f[i][2 * j + 1] = v * c[j] + u * s[j];
         }
@@ -160,7 +178,7 @@ __global__ __launch_bounds__(ROWS_WG) void rows_kernel(SasRowArgs a) {
       if (!in_table) {
         // a position without angles has no rotation: not a number, rather than another's
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[i][e] = __builtin_nanf("");
+        for (int e = 0; e < 8; ++e) f[i][e] = (W)__builtin_nanf("");
       }
     }
   }
@@ -184,12 +202,15 @@ __global__ __launch_bounds__(ROWS_WG) void rows_kernel(SasRowArgs a) {
 
   // fp8 rows: one scale per 128 dims (16 lanes) of the 512 latent dims, or one per index row
   constexpr int SCALE_LANES = OUT == OUT_FP8_MLA ? 16 : G;
-  float amax = 0.0f;
+  float y[8], amax = 0.0f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(f[0][e]));
+  for (int e = 0; e < 8; ++e) {
+    y[e] = (float)f[0][e];
+    amax = fmaxf(amax, fabsf(y[e]));
+  }
   bool bad = false;  // fmaxf drops NaN: a row with one gets a NaN scale
 #pragma unroll
-  for (int e = 0; e < 8; ++e) bad |= f[0][e] != f[0][e];
+  for (int e = 0; e < 8; ++e) bad |= y[e] != y[e];
   if (bad) amax = __builtin_inff();
 #pragma unroll
   for (int off = 1; off < SCALE_LANES; off <<= 1) amax = fmaxf(amax, __shfl_xor(amax, off, 64));
@@ -200,7 +221,7 @@ __global__ __launch_bounds__(ROWS_WG) void rows_kernel(SasRowArgs a) {
     float q[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      q[e] = fminf(fmaxf(f[0][4 * k + e] / scale, -ROWS_E4M3_MAX), ROWS_E4M3_MAX);
+      q[e] = fminf(fmaxf(y[4 * k + e] / scale, -ROWS_E4M3_MAX), ROWS_E4M3_MAX);
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
     w = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
     packed[k] = (uint32_t)w;
@@ -213,7 +234,7 @@ __global__ __launch_bounds__(ROWS_WG) void rows_kernel(SasRowArgs a) {
     if (lane < 8) {
       typename Vec8<T>::type v;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = (T)f[NCH - 1][e];
+      for (int e = 0; e < 8; ++e) v[e] = (T)(float)f[NCH - 1][e];
       *(typename Vec8<T>::type*)(o + 528 + 16 * lane) = v;
     }
   } else if (lane < chunks) {

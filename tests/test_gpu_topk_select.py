@@ -287,3 +287,49 @@ def test_graph_with_other_lengths(rows):
         torch.cuda.synchronize()
         assert torch.equal(out, sparse_topk_indices(**args)), lens
     assert torch.equal(out, want)
+
+
+@requires_gpu
+@pytest.mark.parametrize("n,k", [(40003, 8000), (40003, 30000), (270001, 600), (9001, 8990), (2049, 2048)])
+def test_wide_selections_and_the_longest_rows(n, k):
+    # more ids, or longer rows, than the registers' path takes: the same steps from memory
+    _check(_case(rows=[1, 1], lens=[n, n - 7], heads=3, d=64, k=k, bs=128, seed=n + k))
+
+
+@requires_gpu
+@pytest.mark.parametrize("n", [700, 6000, 20000, 50000])
+def test_uneven_scores(n):
+    # a periodic row (what a sample of it sees is not what it is) and rows with a few scores far
+    # above the rest, so that most of a histogram's range is empty
+    args = _case(rows=[1, 1], lens=[n, n - 100], heads=4, d=64, k=n // 9, bs=64, seed=n)
+    flat, table = args["index_k"].view(-1, 64), args["index_block_table"]
+    j = torch.arange(n - 100)
+    rows0 = (table[0, j // 64] * 64 + j % 64).long()
+    rows1 = (table[1, j // 64] * 64 + j % 64).long()
+    flat[rows0[j % 32 < 4]] *= 1e-3
+    flat[rows1[[3, n // 2, n - 200]]] *= 1e5
+    _check(args)
+
+
+@requires_gpu
+def test_a_nan_key_in_a_long_row():
+    args = _case(rows=[1, 5], lens=[9000, 8500], heads=2, d=64, k=512, bs=64)
+    flat, table = args["index_k"].view(-1, 64), args["index_block_table"]
+    flat[int(table[0, 9]) * 64 + 5, 3] = float("nan")
+    flat[int(table[1, 20]) * 64 + 7, 1] = float("-inf")
+    _check(args)
+
+
+@requires_gpu
+def test_many_rows_take_the_single_wave_path():
+    # from 512 rows of short sequences on a wave owns a row
+    _check(_case(rows=[300, 1, 400], lens=[420, 1900, 401], heads=3, d=64, k=50, bs=16, ratio=1), "many rows")
+    _check(_case(rows=[600], lens=[600], heads=2, d=64, k=40, bs=16, whole=True), "ties in many rows")
+
+
+@requires_gpu
+def test_sequences_without_rows_or_pages():
+    args = _case(rows=[0, 0, 3, 0], lens=[50, 0, 60, 10], heads=4, d=64, k=20)
+    _check(args)
+    args["index_block_table"] = torch.full_like(args["index_block_table"], -1)
+    assert (_check(args) == -1).all()
