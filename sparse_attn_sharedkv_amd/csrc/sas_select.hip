@@ -105,13 +105,13 @@ __device__ inline u32x4 widen_e4m3(u32x2 c) {
   return r;
 }
 
-// The bound on an fp32 score's error: 0 where every score is exactly 0, infinite where it says
-// nothing.
+// The bound on an fp32 score's error: 0 where every score is exactly 0 (no weights, or keys without
+// a bit set: a cache nobody has written), infinite where it says nothing. 2^-110 is above what sums and products below fp32's normal range lose.
 __device__ inline float score_error(const SasSelectArgs& a, float w_norm, float k_norm2) {
+  if (w_norm == 0.0f || k_norm2 == 0.0f) return 0.0f;
   const float err = ((float)a.dim + (float)a.heads / 16.0f + 8.0f) * 1.1920929e-7f * w_norm *
                     (sqrtf(k_norm2) + SEL_TINY);
-  if (k_norm2 == 0.0f || w_norm == 0.0f) return 0.0f;
-  return err <= SEL_MAX ? err : __builtin_inff();
+  return err <= SEL_MAX ? fmaxf(err, 7.7037197775489434e-34f) : __builtin_inff();
 }
 
 // What both kernels know of a launch besides its arguments.
@@ -253,7 +253,11 @@ struct QueryFrags {
         }
       n2 += __shfl_xor(n2, 32, 64);
       const int h = 32 * mt + (lane & 31);
-      if (h < a.heads) s += fabsf(a.weights[(int64_t)t * a.heads + h]) * (sqrtf(n2) + SEL_TINY);
+      if (h < a.heads) {
+        const float w = fabsf(a.weights[(int64_t)t * a.heads + h]);
+        const float v = w * (sqrtf(n2) + SEL_TINY);
+        s += w != 0.0f && v < 7.52e-37f ? 7.52e-37f : v;  // (2^-120: no weight but 0 vanishes)
+      }
     }
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) s += __shfl_xor(s, off, 64);
@@ -287,15 +291,27 @@ struct QueryFrags {
   }
 };
 
+// |k|^2, or the smallest normal number where a key that is not 0 has no square in fp32.
+__device__ inline float norm_kept(float n2, bool zero) { return n2 == 0.0f && !zero ? 1.17549435e-38f : n2; }
+
 template <typename T, int D>
-__device__ inline float key_norm2(const u32x4 k[D / 16]) {
+__device__ inline float key_norm2(const u32x4 k[D / 16], float scale) {
   float n[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
     for (int e = 0; e < 4; ++e) n[e] = Elem<T>::dot2(k[kk][e], n[e]);
-  const float s = (n[0] + n[1]) + (n[2] + n[3]);
-  return s + __shfl_xor(s, 32, 64);
+  float s = (n[0] + n[1]) + (n[2] + n[3]);
+  s += __shfl_xor(s, 32, 64);
+  s *= scale * scale;
+  if (__any(s == 0.0f)) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) bits |= k[kk][0] | k[kk][1] | k[kk][2] | k[kk][3];
+    bits |= __shfl_xor(bits, 32, 64);
+    s = norm_kept(s, (bits & 0x7fff7fffu) == 0 || scale == 0.0f);
+  }
+  return s;
 }
 
 __device__ inline float kept_score(float s) {
@@ -421,8 +437,7 @@ __global__ __launch_bounds__(256, MT <= 2 ? 2 : 1) void score_stream_kernel(SasS
       }
       if (FP8) turn((u + 1) % DEPTH, part);  // the next tile's, under this one's products
       if (norms) {
-        float n2 = key_norm2<T, D>(k);
-        if (FP8) n2 *= sc * sc;
+        const float n2 = key_norm2<T, D>(k, sc);
         if (is) kn = max_nonneg(kn, n2);
       }
       float s = qf.score(k, hf);
@@ -518,13 +533,21 @@ __global__ __launch_bounds__(64 * TILE_WAVES) void score_tile_kernel(SasSelectAr
           k[1] = widen_e4m3<T>(u32x2{held[buf][0][2], held[buf][0][3]});
         }
         float n2 = 0.0f;
+        uint32_t bits = 0;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) n2 = Elem<T>::dot2(k[i][e], n2);
+          for (int e = 0; e < 4; ++e) {
+            n2 = Elem<T>::dot2(k[i][e], n2);
+            bits |= k[i][e];
+          }
 #pragma unroll
-        for (int off = 1; off < PARTS; off <<= 1) n2 += __shfl_xor(n2, off, 64);
+        for (int off = 1; off < PARTS; off <<= 1) {
+          n2 += __shfl_xor(n2, off, 64);
+          bits |= __shfl_xor(bits, off, 64);
+        }
         if (FP8) n2 *= held_scale[buf] * held_scale[buf];
+        n2 = norm_kept(n2, (bits & 0x7fff7fffu) == 0 || (FP8 && held_scale[buf] == 0.0f));
         if (held_ok[buf]) kn = max_nonneg(kn, n2);
       }
       if (!FP8) {

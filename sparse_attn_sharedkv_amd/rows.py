@@ -175,6 +175,8 @@ def norm_rope_heads(q: torch.Tensor, *, positions: Optional[torch.Tensor] = None
         if y is None:
             raise ValueError(f"{who}: out must have heads of contiguous dims aligned to 16 bytes, "
                              "its tokens one stride apart")
+        if _overlaps_itself(tokens, h, d, y):
+            raise ValueError(f"{who}: out overlaps itself")
         if x is None:
             _no_overlap(who, q, out)
             q = _plain(q)
@@ -213,6 +215,17 @@ def _token_view(t: torch.Tensor, h: int, d: int) -> Optional[Tuple[int, int, int
     if dims != 1 or (t.shape[0] > 1 and tokens % 8) or (h > 1 and heads % 8):
         return None
     return at, tokens - tokens % 8, heads - heads % 8  # (strides of one are not used)
+
+
+def _overlaps_itself(tokens: int, h: int, d: int, view: Tuple[int, int, int]) -> bool:
+    _, by_token, by_head = view
+    spans = sorted((s, n) for s, n in ((by_token, tokens), (by_head, h)) if n > 1)
+    reach = d
+    for s, n in spans:
+        if s < reach:
+            return True
+        reach += (n - 1) * s
+    return False
 
 
 def _no_overlap(who: str, x: torch.Tensor, y: torch.Tensor) -> None:
@@ -290,7 +303,10 @@ def append_kv_rope(cache: torch.Tensor, kv: torch.Tensor, slot_mapping: torch.Te
         raise ValueError(f"{who}: cache must be aligned to 16 bytes")
     if n_rows == 0 or cache_rows == 0:
         return
-    stride = kv.stride(0)
+    stride, first = kv.stride(0), kv.data_ptr()
+    if first < at + cache_rows * width * cache.element_size() and \
+            at < first + 2 * ((n_rows - 1) * stride + d):
+        raise ValueError(f"{who}: kv overlaps the cache")
     if kv.stride(-1) != 1 or stride % 8 or kv.data_ptr() % 16:
         kv = _plain(kv)
         stride = d

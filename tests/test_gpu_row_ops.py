@@ -110,6 +110,13 @@ def test_strided_queries_and_outputs():
     with pytest.raises(ValueError, match="overlaps"):
         norm_rope_heads(wide[:5, :512].view(5, 4, 128), positions=pos[:5], cos_sin=table,
                         out=wide[1:, :512].view(5, 4, 128))
+    for out in (torch.zeros(1, 4, 128, dtype=BF, device="cuda").expand(6, 4, 128),
+                torch.zeros(6, 1, 128, dtype=BF, device="cuda").expand(6, 4, 128),
+                torch.zeros(8 * 64 * 8, dtype=BF, device="cuda").as_strided((6, 4, 128), (512, 64, 1))):
+        with pytest.raises(ValueError, match="itself"):
+            norm_rope_heads(q, positions=pos, cos_sin=table, out=out)
+    same = norm_rope_heads(q[:1].expand(6, 4, 128), positions=pos, cos_sin=table, norm_weight=w)
+    assert torch.equal(same[0], want[0]) and not torch.equal(same[1], want[1])
     four = norm_rope_heads(q.reshape(2, 3, 4, 128), positions=pos.view(2, 3).long(), cos_sin=table,
                            norm_weight=w)
     assert torch.equal(four.view(6, 4, 128), want)
@@ -266,6 +273,8 @@ def test_append_odd_inputs():
     append_kv_rope(got, x[:0], slots[:0])
     append_kv_rope(got, x, torch.tensor([1 << 32, (1 << 32) + 1, -1, 16, 1 << 40, -(1 << 40)]).cuda())
     assert torch.equal(got, before)
+    with pytest.raises(ValueError, match="overlaps"):
+        append_kv_rope(got, got.view(16, 128)[2:8], slots)
     nan = x.clone()
     nan[2, 7] = float("nan")
     pages = torch.zeros(2, 8, 1, 132, dtype=torch.uint8, device="cuda")

@@ -333,3 +333,14 @@ def test_sequences_without_rows_or_pages():
     _check(args)
     args["index_block_table"] = torch.full_like(args["index_block_table"], -1)
     assert (_check(args) == -1).all()
+
+
+@requires_gpu
+@pytest.mark.parametrize("heads", [4, 40])
+@pytest.mark.parametrize("keys,weights", [(2.0 ** -66, 1.0), (1.0, 2.0 ** -125), (2.0 ** -40, 2.0 ** -90), (2.0 ** 60, 2.0 ** 40)])
+def test_small_and_large_magnitudes(heads, keys, weights):
+    # squares, products or scores outside fp32's range: the choice is still that of 64 bits
+    args = _case(rows=[1, 5], lens=[400, 300], heads=heads, d=64, k=50, bs=16, seed=heads)
+    args["index_k"] = (args["index_k"].float() * keys).to(BF)
+    args["weights"] = args["weights"] * weights
+    _check(args)
