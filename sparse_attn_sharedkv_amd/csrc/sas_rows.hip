@@ -81,8 +81,9 @@ __global__ __launch_bounds__(ROWS_WG) void rows_kernel(SasRowArgs a) {
   const int lane = threadIdx.x & (G - 1);
   const int64_t row = (int64_t)blockIdx.x * (ROWS_WG / G) + threadIdx.x / G;
   if (row >= (int64_t)a.tokens * a.heads) return;
-  const int t = OUT == OUT_HEADS ? (int)(row / a.heads) : (int)row;
-  const int h = OUT == OUT_HEADS ? (int)(row - (int64_t)t * a.heads) : 0;
+  // (fewer than 2^31 rows: a 32-bit division)
+  const int t = OUT == OUT_HEADS ? (int)((uint32_t)row / (uint32_t)a.heads) : (int)row;
+  const int h = OUT == OUT_HEADS ? (int)row - t * a.heads : 0;
   int64_t slot = 0;
   if (OUT != OUT_HEADS) {
     slot = a.slots[t];

@@ -12,7 +12,7 @@
 // second, a workgroup for each row, finds the topk-th largest and writes the ids.
 //
 // Which rows are chosen does not depend on how the scores were summed. An fp32 score is off by at
-// most E = c W K, c = (D + H + 4) 2^-23, W = sum_h |w_h| |q_h|, K = max_j |k_j| (below), so a row
+// most E = c W K, c = (D + H / 16 + 8) 2^-23, W = sum_h |w_h| |q_h|, K = max_j |k_j| (below), so a row
 // whose fp32 score is more than 2 E above the topk-th largest fp32 score is in, one more than 2 E
 // below it is out, and the few in between are scored again in 64 bits. Ids are therefore those
 // of 64-bit scores for any split of the work, any batch and any tile.
@@ -21,11 +21,11 @@
 // in some order and with some grouping inside the matrix instruction; each addition loses at most
 // 2^-23 of the sum of the magnitudes (a rounding 2^-24, a truncated alignment twice that), so it
 // is off by at most D 2^-23 sum |q_i k_i| <= D 2^-23 |q| |k|. max(0, x) moves no two values
-// further apart. The weighted sum of H terms rounds at most H + 2 times (2^-24 each, of a sum of
-// magnitudes below (1 + small) W K), an fp8 row's scale once more. c has the rest as slack for
-// terms of second order and for the norms' own rounding. 2^-50 is added to each norm for products
-// below fp32's normal range. A bound that is not finite (infinities, NaN, norms beyond fp32)
-// has the whole row scored in 64 bits.
+// further apart. A weighted term passes through at most H / 8 + 1 fused steps of one of eight
+// chains, three sums that join them and an fp8 row's scale, 2^-24 of the magnitudes each:
+// (H / 16 + 2.5) 2^-23. The rest of c is slack for terms of second order and for the norms' own
+// rounding. 2^-50 is added to each norm for products below fp32's normal range. A bound that is
+// not finite (infinities, NaN, norms beyond fp32) has the whole row scored in 64 bits.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -121,7 +121,7 @@ struct SelPlan {
   int chunks;           // workgroups that share a row's keys
   int slices;           // waves that share a piece's keys
   int norms;            // key norms that a piece leaves (one of each wave that has looked at keys)
-  int wq;               // query rows of a workgroup
+  int group;            // query rows of a workgroup
   FastDiv page_div, ratio_div;
   float* w_norm;        // [rows of the pass] W of each row
   float* k_norm;        // [batch][chunks][norms] largest |k|^2 of the keys seen
@@ -332,24 +332,31 @@ __device__ inline int chunk_at(int r, int c) {
   return r * (16 * C) + ((c ^ (r / (16 / C) & (C - 1))) << 4);
 }
 
-// Decode: few query rows a sequence. A workgroup's four waves take wq query rows times 4 / wq
-// slices of a chunk's keys; nothing is shared and there is no barrier. Keys go from memory to
-// registers, the next tile's in flight under the current one's products. Bound by the keys'
-// bytes: a key row is read once for each query row.
+// Decode: few query rows a sequence. A workgroup's four waves take a quarter each of a piece of one
+// query row's keys, and share nothing: no barrier. Whole key rows come from memory into registers
+// (a lane's own parts of its key would be 32 short runs a load), through a wave's own LDS into the
+// operand's layout, and the next tiles' are on their way under the current one's products.
+// Bound by the keys' bytes. Measured with 64 heads of 128 dims: 64 rows over 32768 bf16 keys
+// 118 us, 4.5 TB/s (the loads alone, nothing formed of them, 102 us); 128 rows over 32768 to
+// 131072 fp8 keys 357 us, 3.9 TB/s (alone 300 us). Rows of one sequence read its keys once each:
+// a second row's come out of L2 (64 x 2 rows: 171 us).
+// Tiles in flight: fp8 2, 3 or 1 took 357, 373 and 458 us (3 spill at 64 heads), bf16 1 or 2 took
+// 110 and 122 us.
+constexpr int STREAM_WAVES = 4;
+
 template <bool FP8>
 constexpr int STREAM_DEPTH = FP8 ? 2 : 1;  // tiles of 32 keys that a wave has on their way
 
 template <typename T, bool FP8, int D, int MT>
-__global__ __launch_bounds__(256, MT <= 2 ? 2 : 1) void score_stream_kernel(SasSelectArgs a, SelPlan p) {
-  __shared__ __attribute__((aligned(256))) unsigned char stage[4][32 * (FP8 ? D : 2 * D)];
+__global__ __launch_bounds__(64 * STREAM_WAVES, MT <= 2 ? 2 : 1) void score_stream_kernel(SasSelectArgs a, SelPlan p) {
+  __shared__ __attribute__((aligned(256))) unsigned char stage[STREAM_WAVES][32 * (FP8 ? D : 2 * D)];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 31, hf = lane >> 5;
   const int piece = (int)(blockIdx.x % (unsigned)p.chunks);
-  const int t = p.t_begin + (int)(blockIdx.x / (unsigned)p.chunks) * p.wq + wave % p.wq;
-  if (t >= p.t_end) return;
+  const int t = p.t_begin + (int)(blockIdx.x / (unsigned)p.chunks);
   const RowPos r = locate(a, p, t);
   const int keys = piece_keys(p, r.thr), lo = piece * keys;
   if (r.b < 0 || r.thr <= a.topk || lo >= r.thr) return;
-  const int hi = min(lo + keys, r.thr), slice = wave / p.wq, step = 32 * p.slices;
+  const int hi = min(lo + keys, r.thr), slice = wave, step = 32 * STREAM_WAVES;
 
   QueryFrags<T, D, MT, false> qf;
   qf.load(a, t, lane);
@@ -365,7 +372,7 @@ __global__ __launch_bounds__(256, MT <= 2 ? 2 : 1) void score_stream_kernel(SasS
   // DEPTH tiles on their way from memory, and the pages of the DEPTH behind them
   constexpr int ROW = FP8 ? D : 2 * D, LOADS = ROW / 32, DEPTH = STREAM_DEPTH<FP8>;
   constexpr int C = ROW / 16, R = 64 / C;  // 16-byte chunks of a row, rows of a load
-  const uint32_t page_units = (uint32_t)(a.block_size * (FP8 ? D + 4 : 2 * D) / 16);
+  const uint32_t page_units = (uint32_t)((int64_t)a.block_size * (FP8 ? D + 4 : 2 * D) / 16);
   const unsigned char* lane_keys = (const unsigned char*)a.keys + 16 * (lane % C);
   unsigned char* own = stage[wave];
   u32x4 raw[DEPTH][LOADS];
@@ -385,7 +392,7 @@ __global__ __launch_bounds__(256, MT <= 2 ? 2 : 1) void score_stream_kernel(SasS
       raw[u][q] = *(const u32x4*)(lane_keys + (uint64_t)from * 16);
     }
     if (FP8) {
-      scale[u] = *(const float*)((const unsigned char*)a.keys + (uint64_t)(pg + a.block_size * C) * 16 +
+      scale[u] = *(const float*)((const unsigned char*)a.keys + (uint64_t)(pg + (uint32_t)a.block_size * C) * 16 +
                                  4 * at);
     }
   };
@@ -453,8 +460,12 @@ __global__ __launch_bounds__(256, MT <= 2 ? 2 : 1) void score_stream_kernel(SasS
 }
 
 // Prefill: many query rows a sequence. A workgroup's eight waves own one query row each and
-// share the keys, 64 at a time through LDS (two stages, the next one's loads in flight under the
-// current one's products; fp8 codes are widened on the way in). Bound by the matrix cores.
+// share the keys, 64 at a time through LDS (two stages there, two more on their way in registers;
+// fp8 codes are widened on the way in). Bound by the matrix cores and, as much, by the weighted
+// sums: a 32-key tile of 64 heads is 16 matrix instructions (512 cycles) and some 120 vector ones
+// (480), which two waves a SIMD overlap only in part (matrix cores busy 40 %, vector units 40 %).
+// 8192 causal rows over 2048 keys, 64 heads of 128 dims: 149 us, 870 TFLOP/s. Four waves and
+// 32 keys a stage, twice the workgroups a CU: 172 us; instruction groups forced to alternate: 167.
 // A tile of eight rows that spans sequences takes them one after the other.
 constexpr int TILE_WAVES = 8;
 constexpr int TILE_KEYS = 64;
@@ -622,7 +633,9 @@ __global__ __launch_bounds__(64 * TILE_WAVES) void score_tile_kernel(SasSelectAr
 //   2. those above the bound are taken, those inside it scored in 64 bits and ranked;
 //   3. every id taken is a bit of a map in LDS, from which the ids come out in order.
 // Bound by the latency of these steps, not by bytes, so steps are few and long rows get many
-// waves, while the many short rows of a prefill get one wave each, which needs no barriers.
+// waves, while the many short rows of a prefill get one wave each, which needs no barriers. Of the
+// 29 us that a row of 32768 scores takes, reading it and its bound is 5.5, the topk-th 10.5,
+// the list 1.8, 64-bit scores of the 43 rows inside the bound 9, the ids 1.
 // What does not fit (a bound that is not finite, more equal scores than the lists hold) goes
 // through select_from_memory: the same steps over the scores in memory, as often as it takes.
 
@@ -634,6 +647,9 @@ struct SelSize {
   static constexpr int PARTS = THREADS == 64 ? 1 : SAS_SELECT_MAX_HEADS / 16;
 };
 
+// The workgroup's sums take one barrier each: every use has a row of SelShared::sums of its own.
+enum SelSlot { SLOT_THERE, SLOT_SAMPLE, SLOT_COUNT, SLOT_ABOVE, SLOT_IDS, SLOT_NUM };
+
 template <int THREADS>
 struct SelShared {
   typedef SelSize<THREADS> S;
@@ -641,7 +657,7 @@ struct SelShared {
   float list_x[S::LIST];
   int list_j[S::LIST];
   uint64_t list_key[S::LIST];
-  int sums[8][S::WAVES];  // by SelSlot
+  int sums[SLOT_NUM][S::WAVES];
   int wave_a[S::WAVES], wave_b[S::WAVES];
   float wave_lo[S::WAVES], wave_hi[S::WAVES];
   int close_j[S::LIST];
@@ -762,8 +778,6 @@ __device__ inline float wave_min(float v) {
 }
 __device__ inline float wave_max(float v) { return -wave_min(-v); }
 
-// The workgroup's sums take one barrier each: every use has a row of sh.sums of its own.
-enum SelSlot { SLOT_THERE, SLOT_SAMPLE, SLOT_COUNT, SLOT_ABOVE, SLOT_IDS, SLOT_FREE, SLOT_NUM };
 
 template <int THREADS>
 __device__ inline int block_sum(int v, SelSlot slot, SelShared<THREADS>& sh) {
@@ -857,8 +871,8 @@ struct BinMap {
 // The choice from scores in memory, for what the registers and lists do not hold.
 template <typename T, bool FP8, int THREADS>
 __device__ inline void select_from_memory(const SasSelectArgs& a, const SelPlan& p, int t, int n,
-                                                float err, float* x_of, const int32_t* table,
-                                                SelShared<THREADS>& sh) {
+                                          float err, float* x_of, const int32_t* table,
+                                          SelShared<THREADS>& sh) {
   constexpr int WAVES = THREADS / 64, BINS = SelSize<THREADS>::BINS, LIST = SelSize<THREADS>::LIST;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int k = a.topk;
@@ -1466,14 +1480,21 @@ PassPlan plan_passes(const SasSelectArgs& a) {
   rows = rows < 8 ? 8 : rows / 8 * 8;
   r.rows = (int)(rows < a.tokens ? rows : a.tokens);
   const int64_t per_seq = a.batch > 0 ? (int64_t)a.tokens / a.batch : 0;
+  // From four query rows a sequence on, keys shared through LDS beat a row on its own (32
+  // sequences of 16384 keys, 4 rows: 71 us against 81; at 2 rows the shared kernel has six of
+  // its eight waves idle: 13 sequences, 36 us against 21).
   r.tiles = per_seq >= 4;
-  p.wq = r.tiles ? TILE_WAVES : per_seq >= 2 ? 2 : 1;
-  p.slices = r.tiles ? 1 : 4 / p.wq;
-  p.norms = r.tiles ? TILE_WAVES : p.slices;
-  const int64_t groups = (r.rows + p.wq - 1) / p.wq;
-  // enough workgroups to fill the chip a few times over, of at least 64 keys a slice
+  p.group = r.tiles ? TILE_WAVES : 1;
+  p.slices = r.tiles ? 1 : STREAM_WAVES;
+  p.norms = r.tiles ? TILE_WAVES : STREAM_WAVES;
+  const int64_t groups = (r.rows + p.group - 1) / p.group;
+  // Enough workgroups to fill the chip a few times over, of at least 64 keys a slice. Decode rows,
+  // 1024 / 2048 workgroups: even lengths (64 x 32768 keys) 110 / 118 us, uneven ones (128 x
+  // 32768 to 131072, fp8) 383 / 357 us; even batches are the ones that lose least. A mixed step
+  // of 633 rows with 256 / 512 / 1024: 79 / 66 / 61 us, its first version.
   const int64_t most = (p.width + 64 * p.slices - 1) / (64 * p.slices);
-  const int64_t pieces = ((r.tiles ? 512 : 2048) + groups - 1) / (groups < 1 ? 1 : groups);
+  const int64_t wanted = r.tiles ? 512 : 2048;
+  const int64_t pieces = (wanted + groups - 1) / (groups < 1 ? 1 : groups);
   p.chunks = (int)(pieces < 1 ? 1 : pieces > most ? most : pieces);
   // every part starts on 16 bytes
   const int64_t w_floats = ((int64_t)r.rows + 3) / 4 * 4;
@@ -1523,12 +1544,12 @@ int check_select(const SasSelectArgs* a) {
 
 template <typename T, bool FP8, int D, int MT>
 void launch_scores(const SasSelectArgs& a, const PassPlan& r, const SelPlan& p, hipStream_t st) {
-  const int64_t groups = (p.t_end - p.t_begin + p.wq - 1) / p.wq;
+  const int64_t groups = (p.t_end - p.t_begin + p.group - 1) / p.group;
   const dim3 grid((unsigned)(groups * p.chunks));
   if (r.tiles) {
     hipLaunchKernelGGL((score_tile_kernel<T, FP8, D, MT>), grid, dim3(64 * TILE_WAVES), 0, st, a, p);
   } else {
-    hipLaunchKernelGGL((score_stream_kernel<T, FP8, D, MT>), grid, dim3(256), 0, st, a, p);
+    hipLaunchKernelGGL((score_stream_kernel<T, FP8, D, MT>), grid, dim3(64 * STREAM_WAVES), 0, st, a, p);
   }
 }
 
@@ -1548,12 +1569,15 @@ void launch_pass(const SasSelectArgs& a, const PassPlan& r, const SelPlan& p, hi
   }
   const int rows = p.t_end - p.t_begin;
   const dim3 grid((unsigned)rows);
-  if (a.max_keys <= 2048 && rows >= 512) {
+  // The workgroup of a row. Of many short rows one wave each: 1024 / 1536 / 2048 / 3000 / 6771 rows
+  // of up to 2048 scores take 33 / 33 / 40 / 45 / 71 us with 64 threads and 22 / 34 / 39 / 54 /
+  // 106 us with 256. Up to 8192 scores 256 threads hold a row (32 rows of 4096: 15.4 us, with 1024
+  // threads 17.1); longer rows are sampled first (64 rows of 32768: 32.1 us, all of a row in the
+  // registers of 1024 threads 34.1).
+  if (a.max_keys <= 2048 && rows >= 2048) {
     hipLaunchKernelGGL((select_kernel<T, FP8, 64, 32, false>), grid, dim3(64), 0, st, a, p);
   } else if (a.max_keys <= 8192) {
     hipLaunchKernelGGL((select_kernel<T, FP8, 256, 32, false>), grid, dim3(256), 0, st, a, p);
-  } else if (a.max_keys <= 32768) {
-    hipLaunchKernelGGL((select_kernel<T, FP8, 1024, 32, false>), grid, dim3(1024), 0, st, a, p);
   } else {
     hipLaunchKernelGGL((select_kernel<T, FP8, 1024, 8, true>), grid, dim3(1024), 0, st, a, p);
   }
