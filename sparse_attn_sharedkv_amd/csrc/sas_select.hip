@@ -114,17 +114,26 @@ __device__ inline float score_error(const SasSelectArgs& a, float w_norm, float 
   return err <= SEL_MAX ? fmaxf(err, 7.7037197775489434e-34f) : __builtin_inff();
 }
 
-// What both kernels know of a launch besides its arguments.
+// Sequences of fewer query rows than this have their keys read for each row.
+constexpr int SEL_FEW_ROWS = 4;
+
+// How a score kernel shares a row's keys out.
+struct SelSplit {
+  int chunks;  // workgroups that share a row's keys
+  int slices;  // waves that share a piece's keys
+  int norms;   // key norms that a piece leaves (one of each wave that has looked at keys)
+};
+
+// What the kernels know of a launch besides its arguments.
 struct SelPlan {
   int t_begin, t_end;   // query rows of this pass
   int width;            // scores kept for a row (row stride of the workspace)
-  int chunks;           // workgroups that share a row's keys
-  int slices;           // waves that share a piece's keys
-  int norms;            // key norms that a piece leaves (one of each wave that has looked at keys)
-  int group;            // query rows of a workgroup
+  int few_rows;         // sequences of fewer rows than this go to score_stream_kernel
+  SelSplit few, many;   // of score_stream_kernel, of score_tile_kernel
+  int norm_stride;      // key norms of a sequence
   FastDiv page_div, ratio_div;
   float* w_norm;        // [rows of the pass] W of each row
-  float* k_norm;        // [batch][chunks][norms] largest |k|^2 of the keys seen
+  float* k_norm;        // [batch][norm_stride] largest |k|^2 of the keys seen
   float* score;         // [rows of the pass][width]
 };
 
@@ -132,6 +141,7 @@ struct RowPos {
   int b;     // sequence, -1: a row of no sequence
   int thr;   // keys the row may choose from
   int last;  // first query row behind the sequence's (or behind the run of rows of no sequence)
+  int rows;  // query rows of the sequence
 };
 
 __device__ inline RowPos locate(const SasSelectArgs& a, const SelPlan& p, int t) {
@@ -142,7 +152,7 @@ __device__ inline RowPos locate(const SasSelectArgs& a, const SelPlan& p, int t)
     s = t - b * a.rows_per_seq;
     act_q = a.cu_seqlens_q ? a.cu_seqlens_q[b + 1] - a.cu_seqlens_q[b] : a.rows_per_seq;
     if (act_q > a.rows_per_seq) act_q = a.rows_per_seq;
-    if (s >= act_q) return {-1, 0, (b + 1) * a.rows_per_seq};
+    if (s >= act_q) return {-1, 0, (b + 1) * a.rows_per_seq, 0};
     r.b = b;
     r.last = b * a.rows_per_seq + act_q;
   } else {
@@ -161,9 +171,9 @@ __device__ inline RowPos locate(const SasSelectArgs& a, const SelPlan& p, int t)
         hi = mid;
       }
     }
-    if (lo < 0) return {-1, 0, a.batch > 0 ? a.cu_seqlens_q[0] : a.tokens};
+    if (lo < 0) return {-1, 0, a.batch > 0 ? a.cu_seqlens_q[0] : a.tokens, 0};
     const int first = a.cu_seqlens_q[lo], end = a.cu_seqlens_q[lo + 1];
-    if (t >= end) return {-1, 0, lo + 1 < a.batch ? a.cu_seqlens_q[lo + 1] : a.tokens};
+    if (t >= end) return {-1, 0, lo + 1 < a.batch ? a.cu_seqlens_q[lo + 1] : a.tokens, 0};
     r.b = lo;
     s = t - first;
     act_q = end - first;
@@ -171,6 +181,7 @@ __device__ inline RowPos locate(const SasSelectArgs& a, const SelPlan& p, int t)
   }
   const ItemGeom g = item_geom_div(act_q, a.seqused_kv[r.b], s, -1, 2, p.ratio_div, 0);
   r.thr = min(g.thr, a.max_keys);
+  r.rows = act_q;
   return r;
 }
 
@@ -181,9 +192,9 @@ __device__ inline int thr_at(const SasSelectArgs& a, const SelPlan& p, int t) {
 // Keys of one of a row's pieces: equal shares of the keys it has, in whole steps of 64 keys a
 // slice, so no workgroup of a short sequence in a wide table goes without work before the
 // last pieces do.
-__device__ inline int piece_keys(const SelPlan& p, int thr) {
-  const int unit = 64 * p.slices;
-  return ((thr + p.chunks - 1) / p.chunks + unit - 1) / unit * unit;
+__device__ inline int piece_keys(const SelSplit& sp, int thr) {
+  const int unit = 64 * sp.slices;
+  return ((thr + sp.chunks - 1) / sp.chunks + unit - 1) / unit * unit;
 }
 
 // ---------------------------------------------------------------------------
@@ -351,11 +362,21 @@ template <typename T, bool FP8, int D, int MT>
 __global__ __launch_bounds__(64 * STREAM_WAVES, MT <= 2 ? 2 : 1) void score_stream_kernel(SasSelectArgs a, SelPlan p) {
   __shared__ __attribute__((aligned(256))) unsigned char stage[STREAM_WAVES][32 * (FP8 ? D : 2 * D)];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 31, hf = lane >> 5;
-  const int piece = (int)(blockIdx.x % (unsigned)p.chunks);
-  const int t = p.t_begin + (int)(blockIdx.x / (unsigned)p.chunks);
+  const int piece = (int)(blockIdx.x % (unsigned)p.few.chunks);
+  int t = (int)(blockIdx.x / (unsigned)p.few.chunks);
+  if (p.few_rows == SEL_FEW_ROWS) {
+    // a mixed step: the workgroups are of the rows that short sequences may have
+    const int b = t / (SEL_FEW_ROWS - 1), s = t - b * (SEL_FEW_ROWS - 1);
+    const int first = a.cu_seqlens_q[b], rows = a.cu_seqlens_q[b + 1] - first;
+    if (s >= rows || rows >= SEL_FEW_ROWS) return;
+    t = s + (a.rows_per_seq > 0 ? b * a.rows_per_seq : first);
+    if (t < p.t_begin || t >= p.t_end) return;
+  } else {
+    t += p.t_begin;
+  }
   const RowPos r = locate(a, p, t);
-  const int keys = piece_keys(p, r.thr), lo = piece * keys;
-  if (r.b < 0 || r.thr <= a.topk || lo >= r.thr) return;
+  const int keys = piece_keys(p.few, r.thr), lo = piece * keys;
+  if (r.b < 0 || r.rows >= p.few_rows || r.thr <= a.topk || lo >= r.thr) return;
   const int hi = min(lo + keys, r.thr), slice = wave, step = 32 * STREAM_WAVES;
 
   QueryFrags<T, D, MT, false> qf;
@@ -455,7 +476,7 @@ __global__ __launch_bounds__(64 * STREAM_WAVES, MT <= 2 ? 2 : 1) void score_stre
   if (norms) {
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) kn = max_nonneg(kn, __shfl_xor(kn, off, 64));
-    if (lane == 0) p.k_norm[((int64_t)r.b * p.chunks + piece) * p.norms + slice] = kn;
+    if (lane == 0) p.k_norm[(int64_t)r.b * p.norm_stride + piece * p.few.norms + slice] = kn;
   }
 }
 
@@ -477,10 +498,10 @@ __global__ __launch_bounds__(64 * TILE_WAVES) void score_tile_kernel(SasSelectAr
   __shared__ int key_ok[2][TILE_KEYS];
   __shared__ __attribute__((aligned(16))) float weight[TILE_WAVES][32 * MT];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 31, hf = lane >> 5;
-  const int piece = (int)(blockIdx.x % (unsigned)p.chunks);
+  const int piece = (int)(blockIdx.x % (unsigned)p.many.chunks);
   const int tiles = (p.t_end - p.t_begin + TILE_WAVES - 1) / TILE_WAVES;
   // the last rows of a causal prefill have the most keys: they start first
-  const int t0 = p.t_begin + (tiles - 1 - (int)(blockIdx.x / (unsigned)p.chunks)) * TILE_WAVES;
+  const int t0 = p.t_begin + (tiles - 1 - (int)(blockIdx.x / (unsigned)p.many.chunks)) * TILE_WAVES;
   const int t1 = min(t0 + TILE_WAVES, p.t_end), t = t0 + wave;
   // the thread's part of a stage: bytes [32 part, +32) of native row `row`, or 16 codes
   constexpr int PARTS = 64 * TILE_WAVES / TILE_KEYS;   // 8 threads a row
@@ -493,8 +514,8 @@ __global__ __launch_bounds__(64 * TILE_WAVES) void score_tile_kernel(SasSelectAr
   for (int ts = t0; ts < t1;) {
     const RowPos seg = locate(a, p, ts);
     const int te = max(min(seg.last, t1), ts + 1);
-    const int thr_end = seg.b < 0 ? 0 : thr_at(a, p, te - 1);
-    const int keys = piece_keys(p, thr_end), lo = piece * keys, hi = min(lo + keys, thr_end);
+    const int thr_end = seg.b < 0 || seg.rows < p.few_rows ? 0 : thr_at(a, p, te - 1);
+    const int keys = piece_keys(p.many, thr_end), lo = piece * keys, hi = min(lo + keys, thr_end);
     if (thr_end <= a.topk || lo >= thr_end) {
       ts = te;
       continue;
@@ -617,7 +638,7 @@ __global__ __launch_bounds__(64 * TILE_WAVES) void score_tile_kernel(SasSelectAr
     if (norms) {
 #pragma unroll
       for (int off = 1; off < 64; off <<= 1) kn = max_nonneg(kn, __shfl_xor(kn, off, 64));
-      if (lane == 0) p.k_norm[((int64_t)seg.b * p.chunks + piece) * p.norms + wave] = kn;
+      if (lane == 0) p.k_norm[(int64_t)seg.b * p.norm_stride + piece * p.many.norms + wave] = kn;
     }
     ts = te;
   }
@@ -1199,9 +1220,10 @@ __global__ __launch_bounds__(THREADS, THREADS == 64 ? 5 : 4) void select_kernel(
     }
     float kn = 0.0f;
     {
-      const int thr_end = thr_at(a, p, min(r.last, p.t_end) - 1), keys = piece_keys(p, thr_end);
-      const int parts = (thr_end + keys - 1) / keys * p.norms;
-      const float* kp = p.k_norm + (int64_t)r.b * p.chunks * p.norms;
+      const SelSplit sp = r.rows < p.few_rows ? p.few : p.many;
+      const int thr_end = thr_at(a, p, min(r.last, p.t_end) - 1), keys = piece_keys(sp, thr_end);
+      const int parts = (thr_end + keys - 1) / keys * sp.norms;
+      const float* kp = p.k_norm + (int64_t)r.b * p.norm_stride;
       for (int i = lane; i < parts; i += 64) kn = max_nonneg(kn, kp[i]);
       kn = as_float(__builtin_amdgcn_readlane(
           wave_scan(as_int(kn), 0, [](int a, int b) { return max(a, b); }), 63));
@@ -1466,7 +1488,6 @@ constexpr int64_t SEL_PASS_BYTES = 512ll << 20;
 
 struct PassPlan {
   SelPlan p;
-  bool tiles;          // score_tile_kernel
   int rows;            // query rows of a pass
   int64_t bytes;       // workspace
 };
@@ -1482,23 +1503,30 @@ PassPlan plan_passes(const SasSelectArgs& a) {
   const int64_t per_seq = a.batch > 0 ? (int64_t)a.tokens / a.batch : 0;
   // From four query rows a sequence on, keys shared through LDS beat a row on its own (32
   // sequences of 16384 keys, 4 rows: 71 us against 81; at 2 rows the shared kernel has six of
-  // its eight waves idle: 13 sequences, 36 us against 21).
-  r.tiles = per_seq >= 4;
-  p.group = r.tiles ? TILE_WAVES : 1;
-  p.slices = r.tiles ? 1 : STREAM_WAVES;
-  p.norms = r.tiles ? TILE_WAVES : STREAM_WAVES;
-  const int64_t groups = (r.rows + p.group - 1) / p.group;
+  // its eight waves idle: 13 sequences, 36 us against 21). Where the rows differ by sequence, as
+  // the device alone knows, both kernels are launched and each sequence has one of them: tiles of
+  // eight single rows would take their sequences in turn (a step of 633 rows in 23 sequences, 16
+  // of one row: 54 us by tiles alone, 32 + 8 us by both kernels).
+  const bool even = a.rows_per_seq > 0 && !a.cu_seqlens_q;
+  p.few_rows = even ? (a.rows_per_seq < SEL_FEW_ROWS ? INT32_MAX : 0)
+                    : a.batch == 1 ? (a.tokens < SEL_FEW_ROWS ? INT32_MAX : 0)
+                                   : per_seq <= 2 ? INT32_MAX : SEL_FEW_ROWS;
   // Enough workgroups to fill the chip a few times over, of at least 64 keys a slice. Decode rows,
   // 1024 / 2048 workgroups: even lengths (64 x 32768 keys) 110 / 118 us, uneven ones (128 x
   // 32768 to 131072, fp8) 383 / 357 us; even batches are the ones that lose least. A mixed step
   // of 633 rows with 256 / 512 / 1024: 79 / 66 / 61 us, its first version.
-  const int64_t most = (p.width + 64 * p.slices - 1) / (64 * p.slices);
-  const int64_t wanted = r.tiles ? 512 : 2048;
-  const int64_t pieces = (wanted + groups - 1) / (groups < 1 ? 1 : groups);
-  p.chunks = (int)(pieces < 1 ? 1 : pieces > most ? most : pieces);
+  auto split = [&](int64_t groups, int64_t wanted, int slices, int norms) {
+    const int64_t most = (p.width + 64 * slices - 1) / (64 * slices);
+    const int64_t pieces = (wanted + groups - 1) / (groups < 1 ? 1 : groups);
+    return SelSplit{(int)(pieces < 1 ? 1 : pieces > most ? most : pieces), slices, norms};
+  };
+  p.few = split(p.few_rows == SEL_FEW_ROWS ? a.batch : r.rows, 2048, STREAM_WAVES, STREAM_WAVES);
+  p.many = split((r.rows + TILE_WAVES - 1) / TILE_WAVES, 512, 1, TILE_WAVES);
+  const int few_norms = p.few.chunks * p.few.norms, many_norms = p.many.chunks * p.many.norms;
+  p.norm_stride = few_norms > many_norms ? few_norms : many_norms;
   // every part starts on 16 bytes
   const int64_t w_floats = ((int64_t)r.rows + 3) / 4 * 4;
-  const int64_t k_floats = ((int64_t)a.batch * p.chunks * p.norms + 3) / 4 * 4;
+  const int64_t k_floats = ((int64_t)a.batch * p.norm_stride + 3) / 4 * 4;
   r.bytes = 4 * (w_floats + k_floats + (int64_t)r.rows * p.width);
   p.w_norm = (float*)a.workspace;
   p.k_norm = p.w_norm + w_floats;
@@ -1543,28 +1571,31 @@ int check_select(const SasSelectArgs* a) {
 }
 
 template <typename T, bool FP8, int D, int MT>
-void launch_scores(const SasSelectArgs& a, const PassPlan& r, const SelPlan& p, hipStream_t st) {
-  const int64_t groups = (p.t_end - p.t_begin + p.group - 1) / p.group;
-  const dim3 grid((unsigned)(groups * p.chunks));
-  if (r.tiles) {
-    hipLaunchKernelGGL((score_tile_kernel<T, FP8, D, MT>), grid, dim3(64 * TILE_WAVES), 0, st, a, p);
-  } else {
-    hipLaunchKernelGGL((score_stream_kernel<T, FP8, D, MT>), grid, dim3(64 * STREAM_WAVES), 0, st, a, p);
+void launch_scores(const SasSelectArgs& a, const SelPlan& p, hipStream_t st) {
+  const int64_t rows = p.t_end - p.t_begin, tiles = (rows + TILE_WAVES - 1) / TILE_WAVES;
+  if (p.few_rows < INT32_MAX) {
+    hipLaunchKernelGGL((score_tile_kernel<T, FP8, D, MT>), dim3((unsigned)(tiles * p.many.chunks)),
+                       dim3(64 * TILE_WAVES), 0, st, a, p);
+  }
+  if (p.few_rows > 0) {
+    const int64_t alone = p.few_rows == SEL_FEW_ROWS ? (int64_t)a.batch * (SEL_FEW_ROWS - 1) : rows;
+    hipLaunchKernelGGL((score_stream_kernel<T, FP8, D, MT>), dim3((unsigned)(alone * p.few.chunks)),
+                       dim3(64 * STREAM_WAVES), 0, st, a, p);
   }
 }
 
 template <typename T, bool FP8>
-void launch_pass(const SasSelectArgs& a, const PassPlan& r, const SelPlan& p, hipStream_t st) {
+void launch_pass(const SasSelectArgs& a, const SelPlan& p, hipStream_t st) {
   if (a.max_keys > a.topk) {  // else every row takes all it may see: no scores
     const int mt = (a.heads + 31) / 32;
     if (a.dim == 128) {
-      if (mt == 1) launch_scores<T, FP8, 128, 1>(a, r, p, st);
-      else if (mt == 2) launch_scores<T, FP8, 128, 2>(a, r, p, st);
-      else launch_scores<T, FP8, 128, 4>(a, r, p, st);
+      if (mt == 1) launch_scores<T, FP8, 128, 1>(a, p, st);
+      else if (mt == 2) launch_scores<T, FP8, 128, 2>(a, p, st);
+      else launch_scores<T, FP8, 128, 4>(a, p, st);
     } else {
-      if (mt == 1) launch_scores<T, FP8, 64, 1>(a, r, p, st);
-      else if (mt == 2) launch_scores<T, FP8, 64, 2>(a, r, p, st);
-      else launch_scores<T, FP8, 64, 4>(a, r, p, st);
+      if (mt == 1) launch_scores<T, FP8, 64, 1>(a, p, st);
+      else if (mt == 2) launch_scores<T, FP8, 64, 2>(a, p, st);
+      else launch_scores<T, FP8, 64, 4>(a, p, st);
     }
   }
   const int rows = p.t_end - p.t_begin;
@@ -1617,10 +1648,10 @@ extern "C" int sas_topk_select(const SasSelectArgs* a, void* stream) {
     p.t_end = (int64_t)t + r.rows < a->tokens ? t + r.rows : a->tokens;
     const bool fp8 = a->key_format == SAS_ROW_FP8_INDEX;
     if (a->dtype == SAS_DTYPE_BF16) {
-      fp8 ? sas::launch_pass<__bf16, true>(*a, r, p, st) : sas::launch_pass<__bf16, false>(*a, r, p, st);
+      fp8 ? sas::launch_pass<__bf16, true>(*a, p, st) : sas::launch_pass<__bf16, false>(*a, p, st);
     } else {
-      fp8 ? sas::launch_pass<_Float16, true>(*a, r, p, st)
-          : sas::launch_pass<_Float16, false>(*a, r, p, st);
+      fp8 ? sas::launch_pass<_Float16, true>(*a, p, st)
+          : sas::launch_pass<_Float16, false>(*a, p, st);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) {

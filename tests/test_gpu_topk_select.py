@@ -344,3 +344,30 @@ def test_small_and_large_magnitudes(heads, keys, weights):
     args["index_k"] = (args["index_k"].float() * keys).to(BF)
     args["weights"] = args["weights"] * weights
     _check(args)
+
+
+@requires_gpu
+@pytest.mark.parametrize("dtype,scale", [(H, 2.0 ** -18), (H, 2.0 ** -22), (BF, 2.0 ** -130)])
+def test_subnormal_keys(dtype, scale):
+    # keys below their type's normal range, alone and among ordinary ones
+    args = _case(rows=[1, 5], lens=[400, 300], heads=8, d=128, k=50, bs=16, dtype=dtype, seed=7)
+    plain = args["index_k"].clone()
+    args["index_k"] = (plain.float() * scale).to(dtype)
+    _check(args, "all")
+    some = torch.rand(plain.shape[:3] + (1,)) < 0.5
+    args["index_k"] = torch.where(some, args["index_k"], plain)
+    args["weights"] = -args["weights"].abs()  # (scores at most 0: the small keys' are the largest)
+    _check(args, "some")
+
+
+@requires_gpu
+@pytest.mark.parametrize("rows", [[1, 3, 4, 5, 1, 2, 0, 40, 3], [200] + [1] * 20, [1] * 20 + [9] * 8, [3] * 12, [6, 0, 0, 0]])
+def test_mixed_steps(rows):
+    # short and long row counts in one call: each sequence has the kernel of its own count
+    lens = [n + 37 * (i % 5) + 20 for i, n in enumerate(rows)]
+    _check(_case(rows=rows, lens=lens, heads=20, d=128, k=18, bs=16, seed=len(rows)), str(rows))
+    if max(rows) <= 9:  # the same in a padded batch
+        s = max(rows) + 2
+        args = _case(rows=[s] * len(rows), lens=[n + s for n in lens], heads=5, d=64, k=18, layout="BSND")
+        args["cu_seqlens_q"] = torch.tensor([0] + rows, dtype=torch.int32).cumsum(0).to(torch.int32)
+        _check(args, f"padded {rows}")
