@@ -281,7 +281,7 @@ int sas_kv_fp8_append(const void* src, const int32_t* slot_mapping, void* cache,
 
 /* ---- row operators: norm, rotation, cache append (no reference counterpart) ----------
  * The reference takes rotated queries and written caches as inputs (api.py:129-153); these
- * make them. A row x of `dim` elements becomes, in fp32 and rounded once at the end,
+ * make them. A row x of `dim` elements becomes, in fp32 (fp8 formats: 64 bits) and rounded once,
  *   y[d] = x[d] * w[d] / sqrt(mean(x[0..norm_dim)^2) + eps)  for d < norm_dim, else x[d],
  * then the pairs of dims [rope_offset, rope_offset + rope_dim) turn by the angles of the row's
  * position: (a, b) -> (a cos - b sin, b cos + a sin), pair i being dims (2i, 2i + 1) of the

@@ -8,9 +8,8 @@
 //   (a, b) -> (a cos - b sin, b cos + a sin)
 // with pair i = dims (2i, 2i + 1) of the range (interleaved) or (i, i + R / 2) (halves), and
 // cos / sin from the caller's fp32 table. Everything is in fp32 and rounded once, at the store; rows
-// that end in fp8 are in 64 bits up to the value that is quantized, which a code's coarse steps
-// would otherwise turn an fp32 rounding of into a whole step (16384 rows: no slower, the rows'
-// bytes decide).
+// that end in fp8 are in 64 bits up to their codes, whose coarse steps would otherwise turn an
+// fp32 rounding into a whole step now and then (128 rows of 656 bytes: 4.7 us, in fp32 4.6).
 //
 // Bound by memory: a row is read once and written once. A group of G lanes (8 to 64, the fewest
 // that hold the row at 16 bytes a lane, two or four loads a lane above 512 dims) owns a row, so
@@ -203,31 +202,46 @@ __global__ __launch_bounds__(ROWS_WG) void rows_kernel(SasRowArgs a) {
 
   // fp8 rows: one scale per 128 dims (16 lanes) of the 512 latent dims, or one per index row
   constexpr int SCALE_LANES = OUT == OUT_FP8_MLA ? 16 : G;
-  float y[8], amax = 0.0f;
+  // Dims that nothing has changed are quantized as sas_kv_fp8_append does (fp32 scale and quotient);
+  // others from their 64-bit values, so that only the code's own rounding is left.
+  const bool raw = a.norm_dim == 0 && (a.rope_dim == 0 || (OUT == OUT_FP8_MLA && a.rope_offset >= 512));
+  bool bad = false;  // (the maximum drops NaN: a row with one gets a NaN scale)
+  float y[8], stored;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    y[e] = (float)f[0][e];
-    amax = fmaxf(amax, fabsf(y[e]));
+  for (int e = 0; e < 8; ++e) bad |= f[0][e] != f[0][e];
+  if (raw) {
+    float amax = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf((float)f[0][e]));
+    if (bad) amax = __builtin_inff();
+#pragma unroll
+    for (int off = 1; off < SCALE_LANES; off <<= 1) amax = fmaxf(amax, __shfl_xor(amax, off, 64));
+    stored = amax > 0.0f ? amax / ROWS_E4M3_MAX : 1.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (float)f[0][e] / stored;
+  } else {
+    double amax = 0.0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) amax = fmax(amax, fabs((double)f[0][e]));
+    if (bad) amax = (double)__builtin_inff();
+#pragma unroll
+    for (int off = 1; off < SCALE_LANES; off <<= 1) amax = fmax(amax, __shfl_xor(amax, off, 64));
+    stored = amax > 0.0 ? (float)(amax / (double)ROWS_E4M3_MAX) : 1.0f;
+    const double inv = amax > 0.0 ? (double)ROWS_E4M3_MAX / amax : 1.0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (float)((double)f[0][e] * inv);
   }
-  bool bad = false;  // fmaxf drops NaN: a row with one gets a NaN scale
-#pragma unroll
-  for (int e = 0; e < 8; ++e) bad |= y[e] != y[e];
-  if (bad) amax = __builtin_inff();
-#pragma unroll
-  for (int off = 1; off < SCALE_LANES; off <<= 1) amax = fmaxf(amax, __shfl_xor(amax, off, 64));
-  const float scale = amax > 0.0f ? amax / ROWS_E4M3_MAX : 1.0f;
+  if (!(stored < __builtin_inff())) stored = __builtin_nanf("");
   uint32_t packed[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     float q[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      q[e] = fminf(fmaxf(y[4 * k + e] / scale, -ROWS_E4M3_MAX), ROWS_E4M3_MAX);
+    for (int e = 0; e < 4; ++e) q[e] = fminf(fmaxf(y[4 * k + e], -ROWS_E4M3_MAX), ROWS_E4M3_MAX);
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
     w = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
     packed[k] = (uint32_t)w;
   }
-  const float stored = amax < __builtin_inff() ? scale : __builtin_nanf("");
   if (OUT == OUT_FP8_MLA) {
     unsigned char* o = (unsigned char*)a.out + slot * SAS_FP8_ROW_BYTES;
     *(uint2*)(o + 8 * lane) = make_uint2(packed[0], packed[1]);

@@ -1511,17 +1511,18 @@ PassPlan plan_passes(const SasSelectArgs& a) {
   p.few_rows = even ? (a.rows_per_seq < SEL_FEW_ROWS ? INT32_MAX : 0)
                     : a.batch == 1 ? (a.tokens < SEL_FEW_ROWS ? INT32_MAX : 0)
                                    : per_seq <= 2 ? INT32_MAX : SEL_FEW_ROWS;
-  // Enough workgroups to fill the chip a few times over, of at least 64 keys a slice. Decode rows,
-  // 1024 / 2048 workgroups: even lengths (64 x 32768 keys) 110 / 118 us, uneven ones (128 x
-  // 32768 to 131072, fp8) 383 / 357 us; even batches are the ones that lose least. A mixed step
-  // of 633 rows with 256 / 512 / 1024: 79 / 66 / 61 us, its first version.
+  // Enough workgroups to fill the chip, of at least 64 keys a slice. Decode rows, 1024 / 2048
+  // workgroups: even lengths (64 x 32768 keys) 110 / 118 us, uneven ones (128 x 32768 to 131072,
+  // fp8) 383 / 357 us; even batches are the ones that lose least. Tiles of eight rows, 256 / 512 /
+  // 1024: a mixed step of 633 rows 27 / 33 / 41 us, 1024 rows over 4096 keys 81 / 85 / 98 us, 2048
+  // rows of 128 heads over 8192 keys 733 / 660 / 691 us.
   auto split = [&](int64_t groups, int64_t wanted, int slices, int norms) {
     const int64_t most = (p.width + 64 * slices - 1) / (64 * slices);
     const int64_t pieces = (wanted + groups - 1) / (groups < 1 ? 1 : groups);
     return SelSplit{(int)(pieces < 1 ? 1 : pieces > most ? most : pieces), slices, norms};
   };
   p.few = split(p.few_rows == SEL_FEW_ROWS ? a.batch : r.rows, 2048, STREAM_WAVES, STREAM_WAVES);
-  p.many = split((r.rows + TILE_WAVES - 1) / TILE_WAVES, 512, 1, TILE_WAVES);
+  p.many = split((r.rows + TILE_WAVES - 1) / TILE_WAVES, 256, 1, TILE_WAVES);
   const int few_norms = p.few.chunks * p.few.norms, many_norms = p.many.chunks * p.many.norms;
   p.norm_stride = few_norms > many_norms ? few_norms : many_norms;
   // every part starts on 16 bytes

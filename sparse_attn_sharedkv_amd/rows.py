@@ -10,7 +10,7 @@ somebody wrote. These two make them, each in one pass over the data, in the HIP 
 A row ``x`` of ``D`` dims becomes ``x[d] * w[d] / sqrt(mean(x[:N]**2) + eps)`` for ``d < N``
 (``N = norm_weight.numel()``, the other dims as they are), then the dims
 ``[rope_offset, rope_offset + R)`` are rotated by the angles of the row's position. All of it is
-in fp32 and rounded once, to the output's type. Inputs that require a gradient are refused: the
+in fp32 (in 64 bits for rows that end in fp8) and rounded once, to the output's type. Inputs that require a gradient are refused: the
 library has no backward pass.
 
 fp8 index pages (``[blocks, block_size, 1, D + 4]`` uint8) hold, for a page of ``block_size``
@@ -254,7 +254,7 @@ def append_kv_rope(cache: torch.Tensor, kv: torch.Tensor, slot_mapping: torch.Te
 
     ``cache`` ``[blocks, block_size, 1, width]``, contiguous, decides the format: kv's type with
     ``width = D``; uint8 / float8_e4m3fn with 656 bytes a row for ``D = 576`` bf16 rows (the
-    format of ``append_kv_fp8``, quantized from the fp32 result); uint8 / float8_e4m3fn with
+    format of ``append_kv_fp8``, and its bytes where nothing changes the latent dims); uint8 / float8_e4m3fn with
     ``width = D + 4`` for fp8 index pages, ``D`` 64 or 128. Runs on the current stream of the
     cache's device.
     """
